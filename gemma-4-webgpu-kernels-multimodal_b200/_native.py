@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import weakref
 
 import numpy as np
 
@@ -21,6 +22,7 @@ STATUS_NAMES = {0: "OK", 1: "E_ARG", 2: "E_SHAPE", 3: "E_DTYPE", 4: "E_CUDA", 5:
 _VP = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 _I64 = ctypes.c_int64
 _SIGS = [
     ("g4m_create", _VP, [_VP, _I]),
@@ -40,6 +42,15 @@ _SIGS = [
     ("g4m_vision_embed_images", _I, [_VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, _VP, _VP]),
     ("g4m_resize_rgb", _I, [_VP, _I, _VP, _I, _I, _I, _I, _I, _VP]),
     ("g4m_selftest_wait_timeout", _I, [_VP, _I, ctypes.c_longlong]),
+    ("g4m_fp8_quantize", _I, [_VP, _I, _I, _VP, _I, _I64, _I64, _I, _VP, _VP]),
+    ("g4m_fp8_linear_prepare", _I, [_VP, _I, _VP, _VP, _I, _I, _VP, ctypes.POINTER(_VP)]),
+    ("g4m_fp8_linear_run", _I, [_VP, _VP, _I64, _VP, _I, _I64, _VP]),
+    ("g4m_fp8_linear_free", None, [_VP]),
+    ("g4m_norm_residual", _I, [_VP, _I, _VP, _VP]),
+    ("g4m_rope_frequencies", _I, [_I, _D, _I, _D, _D, _D, _D, ctypes.POINTER(_D), ctypes.POINTER(_D)]),
+    ("g4m_rope_prepare", _I, [_VP, _I, _I, _I, _VP, _D, _I, ctypes.POINTER(_VP)]),
+    ("g4m_rope_run", _I, [_VP, _VP, _VP, _I, _I64, _VP, _I, _VP]),
+    ("g4m_rope_free", None, [_VP]),
     ("g4m_vision_embed_batch", _I, [_VP, _I, _VP, _I, _I, _I, _I, _VP, _VP, _VP]),
     ("g4m_vision_embed_device", _I, [_VP, _I, _I, _VP, _I, _I, _I, _I, _VP, _VP]),
     ("g4m_vision_debug_hidden", _I, [_VP, _I, _I, _VP, ctypes.c_size_t]),
@@ -56,6 +67,32 @@ _SIGS = [
     ("g4m_kernel_launches", ctypes.c_longlong, []),
     ("g4m_version", ctypes.c_char_p, []),
 ]
+
+# element types, gated activations and frequency scalings (enums of include/g4m.h)
+F32, BF16, F16 = 0, 1, 2
+ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "banded": 2, "yarn": 3}
+
+
+class Fp8Rows(ctypes.Structure):
+    """g4m_fp8_rows: device pointers of e4m3 codes and their block scales."""
+    _fields_ = [("codes", _VP), ("ldc", _I64), ("scales", _VP), ("lds", _I64)]
+
+
+class NormArgs(ctypes.Structure):
+    """g4m_norm_args."""
+    _fields_ = [("rows", _I64), ("d", ctypes.c_int32), ("dtype", ctypes.c_int32), ("h_dtype", ctypes.c_int32), ("eps", _F),
+                ("y", _VP), ("ldy", _I64), ("w_post", _VP), ("norm_post", ctypes.c_int32), ("norm_pre", ctypes.c_int32),
+                ("gate", _VP), ("ldg", _I64), ("rows_per_gate", _I64), ("branch_scale", _F), ("res_scale", _F),
+                ("h", _VP), ("ldh", _I64), ("h_out", _VP), ("ldh_out", _I64), ("w_pre", _VP), ("n_out", _VP),
+                ("ldn", _I64), ("out", Fp8Rows)]
+
+
+class RopeView(ctypes.Structure):
+    """g4m_rope_view."""
+    _fields_ = [("x", _VP), ("token_stride", _I64), ("head_stride", _I64), ("out", _VP), ("out_token_stride", _I64),
+                ("out_head_stride", _I64), ("heads", ctypes.c_int32)]
+
 
 _lib = None
 
@@ -111,9 +148,12 @@ class Context:
             self.h = L.g4m_create(None, 0)
         if not self.h:
             raise G4MError(4, last_error())
+        self._handles = weakref.WeakSet()  # linears and rotary tables, freed before the context
 
     def close(self):
         if getattr(self, "h", None):
+            for handle in list(getattr(self, "_handles", ())):
+                handle.close()
             lib().g4m_destroy(self.h)
             self.h = None
 
@@ -284,6 +324,108 @@ class Context:
                                            ptr(lengths), sampling_rate, layer_count, int(max_samples),
                                            ctypes.c_void_p(out_ptr), ptr(rows), ctypes.c_void_p(stream) if stream else None))
         return rows
+
+    def fp8_quantize(self, x: int, dtype: int, ldx: int, rows: int, d: int, codes: int, ldc: int, scales: int, lds: int,
+                     act="none", stream: int = 0, device=0) -> None:
+        """g4m_fp8_quantize on device pointers; act: "none", "silu" or "gelu"."""
+        check(lib().g4m_fp8_quantize(self.h, device, ACTIVATIONS[act], x, dtype, ldx, rows, d,
+                                     ctypes.byref(Fp8Rows(codes, ldc, scales, lds)), stream or None))
+
+    def norm_residual(self, args: NormArgs, stream: int = 0, device=0) -> None:
+        """g4m_norm_residual; args as norm_args() builds them."""
+        check(lib().g4m_norm_residual(self.h, device, ctypes.byref(args), stream or None))
+
+    def fp8_linear(self, w, w_scales, bias=None, device=0) -> "Fp8Linear":
+        """Resident 8-bit float linear: w uint8 e4m3 codes [out, in], w_scales
+        float32 [ceil(out / 128), ceil(in / 128)], bias float32 [out]."""
+        return Fp8Linear(self, w, w_scales, bias, device)
+
+    def rope(self, head_dim: int, inv_freq, interleaved=False, attention_scale=1.0, device=0) -> "Rope":
+        """Rotary positions on the first 2 * len(inv_freq) elements of each head."""
+        return Rope(self, head_dim, inv_freq, interleaved, attention_scale, device)
+
+
+class _Handle:
+    """A resident object of a context; close() frees it, at the latest when the context closes."""
+    _free = ""
+
+    def __init__(self, ctx):
+        if not ctx.h:
+            raise G4MError(1, "the context is closed")
+        self._h = ctypes.c_void_p()
+        ctx._handles.add(self)
+        self._ctx = ctx
+
+    def close(self):
+        if getattr(self, "_h", None):
+            getattr(lib(), self._free)(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Fp8Linear(_Handle):
+    _free = "g4m_fp8_linear_free"
+
+    def __init__(self, ctx, w, w_scales, bias=None, device=0):
+        super().__init__(ctx)
+        w = np.ascontiguousarray(w)
+        if w.dtype != np.uint8 or w.ndim != 2:
+            raise ValueError("w must be uint8 e4m3 codes [out, in]")
+        self.out_features, self.in_features = w.shape
+        s = np.ascontiguousarray(w_scales, dtype=np.float32)
+        want = (-(-self.out_features // 128), -(-self.in_features // 128))
+        if s.shape != want:
+            raise ValueError(f"w_scales must be float32 {list(want)}, one for each 128 x 128 block")
+        b = None if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
+        if b is not None and b.shape != (self.out_features,):
+            raise ValueError("bias must be float32 [out]")
+        check(lib().g4m_fp8_linear_prepare(ctx.h, device, ptr(w), ptr(s), self.out_features, self.in_features,
+                                           None if b is None else ptr(b), ctypes.byref(self._h)))
+
+    def run(self, codes: int, ldc: int, scales: int, lds: int, rows: int, y: int, y_dtype: int, ldy: int,
+            stream: int = 0) -> None:
+        """g4m_fp8_linear_run on device pointers."""
+        check(lib().g4m_fp8_linear_run(self._h, ctypes.byref(Fp8Rows(codes, ldc, scales, lds)), rows, y, y_dtype, ldy,
+                                       stream or None))
+
+
+class Rope(_Handle):
+    _free = "g4m_rope_free"
+
+    def __init__(self, ctx, head_dim, inv_freq, interleaved=False, attention_scale=1.0, device=0):
+        super().__init__(ctx)
+        f = np.ascontiguousarray(inv_freq, dtype=np.float64).reshape(-1)
+        check(lib().g4m_rope_prepare(ctx.h, device, head_dim, 2 * f.size, ptr(f), float(attention_scale), int(interleaved),
+                                     ctypes.byref(self._h)))
+
+    def run(self, q: RopeView, k, dtype: int, tokens: int, positions: int, pos_bits=64, stream: int = 0) -> None:
+        """g4m_rope_run: q and (or None) k as rope_view() builds them, positions a device pointer."""
+        check(lib().g4m_rope_run(self._h, ctypes.byref(q), None if k is None else ctypes.byref(k), dtype, tokens, positions,
+                                 pos_bits, stream or None))
+
+
+def norm_args(**fields) -> NormArgs:
+    """g4m_norm_args; fields left out are 0 / NULL, the scales 1, rows_per_gate
+    1, and codes, ldc, scales, lds name the 8-bit output."""
+    out = Fp8Rows(*(fields.pop(k, 0) for k in ("codes", "ldc", "scales", "lds")))
+    return NormArgs(**{"branch_scale": 1.0, "res_scale": 1.0, "rows_per_gate": 1, **fields, "out": out})
+
+
+def rope_view(x: int, token_stride: int, head_stride: int, out: int, out_token_stride: int, out_head_stride: int,
+              heads: int) -> RopeView:
+    return RopeView(x, token_stride, head_stride, out, out_token_stride, out_head_stride, heads)
+
+
+def rope_frequencies(rotary: int, theta: float, scaling="none", factor=1.0, low=1.0, high=32.0, trained=1.0):
+    """(float64 [rotary / 2] radians per position, attention scale) of g4m_rope_frequencies."""
+    f, m = (ctypes.c_double * max(rotary // 2, 1))(), ctypes.c_double()
+    check(lib().g4m_rope_frequencies(rotary, theta, ROPE_SCALINGS[scaling], factor, low, high, trained, f, ctypes.byref(m)))
+    return np.array(f), m.value
 
 
 def image_token_layout(height: int, width: int, patch_size: int, max_soft_tokens: int, pooling_kernel_size: int):

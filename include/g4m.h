@@ -106,6 +106,138 @@ G4M_API void g4m_linear_free(g4m_linear* lin);
  * one device race and must be serialised by the caller. */
 G4M_API int g4m_linear_run_noalloc(g4m_linear* lin, const float* x_dev, int rows, float* y_dev, void* stream);
 
+/* ------------------------------------- 8-bit float linears and row operators */
+
+/* Operators on device memory that a transformer layer chains around its
+ * projections: a residual norm that emits the next projection's 8-bit
+ * operand, a quantiser (with an optional gated activation) that emits one, a
+ * linear over 8-bit float weights that reads it, and rotary positions on the
+ * query and key heads it produces.  No reference counterpart: the reference's
+ * linears are integer (src/kernels/qat.ts), its norms and rotary positions
+ * live inside the towers (src/vision/kernels.ts:5-73).
+ *
+ * Common rules.  Every call is asynchronous on `stream` (NULL = the device's
+ * legacy default stream) of device `device_index` of the context, allocates
+ * nothing, keeps nothing between calls, can be captured into a graph, and
+ * leaves the calling thread's current device as it was; calls on different
+ * streams may overlap.  Row strides (ld*) are in elements, >= the row's
+ * width, any alignment; pointers need the alignment of their element type
+ * (G4M_E_ARG otherwise), 16-byte aligned rows are faster.  Zero rows are
+ * G4M_OK and launch nothing.  Nothing outside the stated rows and columns is
+ * written.  Inputs and outputs must not overlap except where stated. */
+
+enum g4m_dtype { G4M_F32 = 0, G4M_BF16 = 1, G4M_F16 = 2 };
+
+/* Rows of 8-bit floats (e4m3) with one f32 scale for each 128 columns of a
+ * row: value(r, c) = codes[r * ldc + c] * scales[(c / 128) * lds + r].
+ * codes is 16-byte aligned and ldc a multiple of 16 (the linear fetches the
+ * rows by TMA); scales hold ceil(columns / 128) runs of lds >= rows floats.
+ * The quantising operators choose scale = max(amax, 2^-96) / 448 from the
+ * block's largest magnitude and code = e4m3(value / scale), to nearest even.
+ * A block that holds a NaN or an infinity gets a NaN scale and NaN codes. */
+typedef struct g4m_fp8_rows {
+  uint8_t* codes;
+  int64_t ldc;
+  float* scales;
+  int64_t lds;
+} g4m_fp8_rows;
+
+enum g4m_act {
+  G4M_ACT_NONE = 0,      /* v = x,                   x [rows][d] */
+  G4M_ACT_SILU = 1,      /* v = silu(x0) * x1,       x [rows][2 d]: x0 | x1 */
+  G4M_ACT_GELU_TANH = 2  /* v = gelu_tanh(x0) * x1,  x [rows][2 d]: x0 | x1 */
+};
+
+/* Quantise v (see g4m_act; computed in f32) into out's rows x d codes and
+ * scales.  d >= 1, any value. */
+G4M_API int g4m_fp8_quantize(g4m_ctx* ctx, int device_index, int act, const void* x, int dtype, int64_t ldx, int64_t rows,
+                             int d, const g4m_fp8_rows* out, void* stream);
+
+/* Resident 8-bit float linear.  w: e4m3 codes [out][in]; w_scales: f32
+ * [ceil(out/128)][ceil(in/128)], one per 128 x 128 block; bias: f32 [out] or
+ * NULL; host pointers.  Free a linear before its context is destroyed. */
+typedef struct g4m_fp8_linear g4m_fp8_linear;
+G4M_API int g4m_fp8_linear_prepare(g4m_ctx* ctx, int device_index, const uint8_t* w, const float* w_scales, int out, int in,
+                                   const float* bias, g4m_fp8_linear** out_linear);
+/* y[r][o] = sum over blocks k of 128 columns of
+ *             (sum of code products in block k) * scale_x[k][r] * w_scales[o / 128][k]   (+ bias[o])
+ * summed in f32, rounded once to y_dtype.  x holds `rows` rows of `in` columns. */
+G4M_API int g4m_fp8_linear_run(g4m_fp8_linear* lin, const g4m_fp8_rows* x, int64_t rows, void* y, int y_dtype, int64_t ldy,
+                               void* stream);
+G4M_API void g4m_fp8_linear_free(g4m_fp8_linear* lin);
+
+/* Residual update between two blocks, one pass over the rows, in f32:
+ *   b  = norm_post ? y / sqrt(mean(y^2) + eps) * w_post : y          (0 without y)
+ *   h' = res_scale * (h + branch_scale * gate * b)                   (h 0 and gate 1 where absent)
+ *   n  = norm_pre  ? h' / sqrt(mean(h'^2) + eps) * w_pre : h'
+ * n comes from h' before its rounding to h_dtype.  y, gate and n_out have
+ * type `dtype`, h and h_out `h_dtype`; w_post and w_pre are f32 [d] or NULL
+ * (all ones).  Row r uses gate row r / rows_per_gate (one gate row for each
+ * clip, image or token; rows_per_gate >= rows: one for all).  Any of h_out,
+ * n_out and out may be absent (NULL; codes NULL), not all of them.  h_out may
+ * be h itself and n_out may be y itself (same pointer and stride).
+ * 1 <= d <= 16384 (G4M_E_UNSUPPORTED above). */
+typedef struct g4m_norm_args {
+  int64_t rows;
+  int32_t d;
+  int32_t dtype, h_dtype;
+  float eps;
+  const void* y;
+  int64_t ldy;
+  const float* w_post;
+  int32_t norm_post, norm_pre;
+  const void* gate;
+  int64_t ldg, rows_per_gate;
+  float branch_scale, res_scale;
+  const void* h;
+  int64_t ldh;
+  void* h_out;
+  int64_t ldh_out;
+  const float* w_pre;
+  void* n_out;
+  int64_t ldn;
+  g4m_fp8_rows out;
+} g4m_norm_args;
+G4M_API int g4m_norm_residual(g4m_ctx* ctx, int device_index, const g4m_norm_args* args, void* stream);
+
+/* Rotary positions.  Pair j of a head turns by position * inv_freq[j]:
+ *   (u, v) -> scale * (u cos - v sin, v cos + u sin)
+ * with (u, v) = elements (j, j + rotary/2) of the head (interleaved == 0) or
+ * (2 j, 2 j + 1) (interleaved != 0), j < rotary/2; elements from `rotary` on
+ * pass through unscaled.  The angle is formed modulo one turn from a 64-bit
+ * fixed-point frequency, so far positions lose nothing. */
+enum g4m_rope_scaling {
+  G4M_ROPE_NONE = 0,    /* theta^(-2 j / rotary) */
+  G4M_ROPE_LINEAR = 1,  /* the same / factor */
+  G4M_ROPE_BANDED = 2,  /* pairs with under `low` turns in `trained` positions / factor, over `high` kept, blended between */
+  G4M_ROPE_YARN = 3     /* the same split as a ramp over the pair index; attention scale 0.1 ln(factor) + 1 */
+};
+/* Host helper: fills inv_freq[rotary / 2] and *attention_scale. */
+G4M_API int g4m_rope_frequencies(int rotary, double theta, int scaling, double factor, double low, double high,
+                                 double trained, double* inv_freq, double* attention_scale);
+
+typedef struct g4m_rope g4m_rope;
+/* head_dim <= 1024; rotary even, 2 <= rotary <= head_dim; inv_freq: host,
+ * [rotary / 2], finite, radians per position.  Free before the context. */
+G4M_API int g4m_rope_prepare(g4m_ctx* ctx, int device_index, int head_dim, int rotary, const double* inv_freq,
+                             double scale, int interleaved, g4m_rope** out_rope);
+
+/* Heads of one projection: element e of head a of token t is at
+ * x[t * token_stride + a * head_stride + e].  out may be x itself with equal
+ * strides (elements that pass through are then left untouched). */
+typedef struct g4m_rope_view {
+  const void* x;
+  int64_t token_stride, head_stride;
+  void* out;
+  int64_t out_token_stride, out_head_stride;
+  int32_t heads;
+} g4m_rope_view;
+/* Turns the heads of q and, unless NULL, of k in one launch.  positions:
+ * device array of `tokens` int32 (pos_bits 32) or int64 (64), any sign. */
+G4M_API int g4m_rope_run(g4m_rope* rope, const g4m_rope_view* q, const g4m_rope_view* k, int dtype, int64_t tokens,
+                         const void* positions, int pos_bits, void* stream);
+G4M_API void g4m_rope_free(g4m_rope* rope);
+
 /* ------------------------------------------------------------- vision */
 
 /* Image embeddings for n images of one size (computeGemma4VisionImageEmbeddings,
