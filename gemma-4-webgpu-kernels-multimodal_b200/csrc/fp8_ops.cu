@@ -178,14 +178,21 @@ int g4m_fp8_linear_prepare(g4m_ctx* ctx, int di, const uint8_t* w, const float* 
     if (!device_ok(ctx, di) || !w || !w_scales || !out_linear || in <= 0 || out <= 0) return fail(G4M_E_ARG, "bad argument");
     Device& d = *ctx->devs[di];
     DeviceGuard guard(d.id);
-    const size_t blocks = ((size_t)in + kFp8Block - 1) / kFp8Block, oblocks = ((size_t)out + kFp8Block - 1) / kFp8Block;
     g4m_fp8_linear* L = new g4m_fp8_linear();
     L->d = &d;
     L->dev = d.id;
     L->in = in;
     L->out = out;
-    if (!to_device(&L->w, w, (size_t)out * in) || !to_device(&L->sw, w_scales, blocks * oblocks) ||
-        (bias && !to_device(&L->bias, bias, (size_t)out))) {
+    uint8_t* raw = nullptr;
+    const bool ok = fp8_gemm_setup() == cudaSuccess && to_device(&raw, w, (size_t)out * in) &&
+                    cudaMalloc(&L->w, fp8_weight_bytes(out, in)) == cudaSuccess &&
+                    fp8_weight_tiles(raw, out, in, L->w, cudaStreamLegacy) == cudaSuccess &&
+                    to_device(&L->sw, w_scales, (size_t)(fp8_blocks(out) * fp8_blocks(in))) &&
+                    (!bias || to_device(&L->bias, bias, (size_t)out)) &&
+                    cudaStreamSynchronize(cudaStreamLegacy) == cudaSuccess;
+    if (raw) cudaFree(raw);
+    if (!ok) {
+      (void)cudaGetLastError();
       g4m_fp8_linear_free(L);
       return fail(G4M_E_CUDA, "8-bit float linear: weight upload failed");
     }
@@ -221,9 +228,10 @@ int g4m_fp8_linear_run(g4m_fp8_linear* L, const g4m_fp8_rows* x, int64_t rows, v
     a.bias = L->bias;
     a.y = y;
     a.y_dtype = y_dtype;
+    a.y_vec = rows16(y, ldy, dtype_size(y_dtype));
     a.ldy = ldy;
     a.err = d.err;
-    G4M_RUN("fp8_gemm", fp8_gemm(a, st));
+    G4M_RUN("fp8_gemm", fp8_gemm(a, L->dev, st));
     return G4M_OK;
   });
 }

@@ -38,21 +38,33 @@ struct RopeArgs {
 };
 cudaError_t rope_run(RopeArgs a, cudaStream_t st);
 
+// Weights live in HBM as the tiles the tensor core reads: 128 outputs x 128
+// columns of codes, 16 KB each, in the 128-byte-swizzled order of shared
+// memory, [output block][column block], zeros past the edges.  A tile is one
+// contiguous copy.  The output blocks are padded to an even number.
+constexpr int kFp8TileBytes = kFp8Block * kFp8Block;
+inline long fp8_blocks(long n) { return (n + kFp8Block - 1) / kFp8Block; }
+inline long fp8_weight_bytes(long out, long in) { return (fp8_blocks(out) + 1) / 2 * 2 * fp8_blocks(in) * kFp8TileBytes; }
+// w: codes [out][in] on the device.
+cudaError_t fp8_weight_tiles(const uint8_t* w, int out, int in, uint8_t* tiles, cudaStream_t st);
+
 struct Fp8GemmArgs {
   long rows;
   int in, out;
-  const uint8_t* x;
+  const uint8_t* x;  // codes [rows][ldx], fetched through a tensor map
   long ldx;
-  const float* sx;
+  const float* sx;   // [blocks of in][lds]
   long lds;
-  const uint8_t* w;
-  const float* sw;
+  const uint8_t* w;  // tiles
+  const float* sw;   // [blocks of out][blocks of in]
   const float* bias;
   void* y;
-  int y_dtype;
+  int y_dtype, y_vec;  // y_vec: rows of y start on 16-byte boundaries
   long ldy;
   int* err;
 };
-cudaError_t fp8_gemm(const Fp8GemmArgs& a, cudaStream_t st);
+// Once per device before the first fp8_gemm: shared-memory limits (loads the kernels, too).
+cudaError_t fp8_gemm_setup();
+cudaError_t fp8_gemm(const Fp8GemmArgs& a, int dev, cudaStream_t st);
 
 }  // namespace g4m

@@ -695,7 +695,23 @@ bool make_tmap_f16_any(CUtensorMap* map, const void* base, uint64_t rows, uint64
   return r == CUDA_SUCCESS;
 }
 
-static int g_num_sms(int dev) {
+// 8-bit matrix [rows, cols], any cols, 16-byte-multiple row pitch: box 128
+// columns x box_rows rows, 128B swizzle; zeros past the edges.
+bool make_tmap_u8_pitch(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch,
+                        uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || !base || pitch % 16 != 0 || pitch < cols || (reinterpret_cast<uintptr_t>(base) % 16) != 0) return false;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
+int g_num_sms(int dev) {
   static int cache[64] = {0};
   if (dev < 0 || dev >= 64) return 148;
   if (!cache[dev]) {
