@@ -29,15 +29,61 @@ namespace g4m {
 // e4m3 A and B (K-major), f32 D: the format fields are those of fp16 (0).
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int m, int n) { return idesc_f16_f32(m, n); }
 
-// D[tmem] (+)= A[smem] * B[smem]^T, kind::f8f6f4, K = 32 codes per instruction.
-template <bool ACC>
-__device__ __forceinline__ void mma_fp8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+// One 128-column block: D[tmem] = A[smem] * B[smem]^T (kind::f8f6f4, four
+// MMAs of K = 32 codes), then an arrival on `bar` when they are done.  Whole
+// warp; one elected lane issues.  With the warp converged the descriptors
+// stay in uniform registers: 157 cycles for the five instructions, where a
+// single-lane branch takes 228.
+__device__ __forceinline__ void mma_block(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a1, b1, a2, b2, a3, b3;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\t"
+      "add.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
+      "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
+      "setp.ne.b32 p, 0, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, p;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Whole warp: the elected lane's arrival on `bar` once its MMAs so far are done.
+__device__ __forceinline__ void mma_commit_elected(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// Whether the phase is complete, without waiting (try_wait may suspend the thread).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "n"(ACC ? 1 : 0)
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
+  return ok != 0;
+}
+
+// Bounded wait of a whole warp: the same answer in every lane.  A test takes
+// 75-140 cycles even when the phase is complete, so loops test the next
+// iteration's barrier early (`ready`, from mbar_test) and only read the
+// answer here.
+__device__ __forceinline__ bool warp_wait(bool ready, uint64_t* bar, uint32_t parity, int* err, int code,
+                                          volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, ready)) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code, abort_flag));
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code, volatile int* abort_flag) {
+  return warp_wait(mbar_try_wait(smem_u32(bar), parity), bar, parity, err, code, abort_flag);
 }
 
 // 16 columns of this warp's lanes; the values are there after tmem_wait16.
@@ -58,22 +104,86 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
                :
                : "memory");
 }
+// The same for two sets.
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[2][16]) {
+  tmem_wait16(r[0]);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[1][i])::"memory");
+}
+
+// Pairs of f32 in one register pair: one instruction for two fma.  The f32
+// pipe takes two cycles for it, so the gain is in issue slots, which the
+// waiting warps need.
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t pack_u32x2(uint32_t a, uint32_t b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+  return v;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+// acc += x * s, elementwise, each rounded to nearest.
+__device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t x, uint64_t s) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(s));
+}
+
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
+// A tile of this CTA's shared memory to global memory (the map's box and swizzle);
+// rows and columns past the tensor's edges are not written.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// This thread's stores have read their shared memory / are complete.
+__device__ __forceinline__ void tma_store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// 4 bytes from global to shared memory without a register; zero unless `valid`.
+__device__ __forceinline__ void cp_async4(float* dst, const float* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-// The float at this CTA's shared address `addr` in the cluster's CTA `rank`.
-__device__ __forceinline__ float cluster_ld(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+// Orders nothing but the arrival itself (a release would wait for this thread's global stores).
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// Shared address `addr` of this CTA in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_map(uint32_t addr, uint32_t rank) {
   uint32_t remote;
-  float v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
+  return remote;
+}
+// Copies `bytes` (a multiple of 16) of this CTA's shared memory into that of a
+// CTA of the cluster, where they count towards the phase of a barrier.  One
+// copy per CTA: an asynchronous store per thread and row cost 400 cycles each
+// on the barrier's account.
+__device__ __forceinline__ void cluster_push(uint32_t remote, const void* src, uint32_t bytes, uint32_t remote_bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(remote),
+               "r"(smem_u32(src)), "r"(bytes), "r"(remote_bar)
+               : "memory");
 }
 
 // The producer's waits for copies that nobody has consumed after a timeout.
@@ -96,9 +206,15 @@ struct ManyCfg {
   static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = 4;
-  static constexpr int EPI_STAGE = 4096;  // per epilogue warp: a 32-row x 128-byte store block
-  static constexpr int THREADS = 64 + 256;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 8 * EPI_STAGE + 1024;
+  static constexpr int EPI_STAGE = 2048;  // per epilogue warp: a 32-row x 64-byte block on its way to y
+  // One warpgroup for the producer, the MMA issuer and two idle warps, four
+  // for the epilogue: a block's waits, scales and arrivals cost each warp as
+  // many cycles as its sums, so four warps per scheduler take turns.  The
+  // registers of a launch at 96 a thread are shared out as 32 and 112:
+  // 128 * 32 + 512 * 112 <= 640 * 96.
+  static constexpr int EPI_WARPS = 16, THREADS = 128 + 32 * EPI_WARPS;
+  static constexpr int COLS = BN / (EPI_WARPS / 4);  // columns of one epilogue warp
+  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * EPI_STAGE + 1024;
   static_assert(SMEM + 1024 <= 232448, "over 227 KB of shared memory");
   static constexpr int GROUP_M = 16;      // row blocks that share the output blocks in L2
 };
@@ -112,41 +228,37 @@ __device__ __forceinline__ void tile_of(int tile, int tiles_m, int tiles_n, int&
 }
 
 __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
-    fp8_gemm_many_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ Fp8GemmArgs a) {
+    fp8_gemm_many_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap my,
+                         const __grid_constant__ Fp8GemmArgs a) {
   using C = ManyCfg;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[C::STAGES], bar_empty[C::STAGES], bar_accf[2], bar_acce[2];
+  __shared__ __align__(8) uint64_t bar_full[C::STAGES], bar_done[C::STAGES], bar_acce[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_flag, skip;
+  __shared__ int abort_flag;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kblocks = (a.in + kFp8Block - 1) / kFp8Block, oblocks = (a.out + kFp8Block - 1) / kFp8Block;
   const int tiles_m = (int)((a.rows + C::BM - 1) / C::BM), tiles_n = (oblocks + 1) / 2, tiles = tiles_m * tiles_n;
 
   if (threadIdx.x == 0) {
-    skip = *reinterpret_cast<volatile int*>(a.err) != 0;
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&bar_full[s], 1);
-      mbar_init(&bar_empty[s], 1);
+      mbar_init(&bar_done[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&bar_accf[b], 1);
-      mbar_init(&bar_acce[b], 8);
-    }
+    for (int b = 0; b < 2; ++b) mbar_init(&bar_acce[b], C::EPI_WARPS);
     abort_flag = 0;
     fence_mbar_init();
-    prefetch_tmap(&mx);
   }
-  __syncthreads();
-  if (skip) return;  // an earlier kernel on this device already failed
+  if (warp == 0 && lane == 0) prefetch_tmap(&mx);
   if (warp == 1) tmem_alloc(&tmem_slot, 2 * C::BN);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    if (warp == 0 && lane == 0) {
       uint32_t it = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
@@ -155,7 +267,10 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         const uint8_t* w = a.w + (long)2 * nb * kblocks * kFp8TileBytes;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % C::STAGES;
-          if (!mbar_wait(&bar_empty[s], ((it / C::STAGES) & 1) ^ 1, a.err, kErrWaitEmpty, &abort_flag)) {
+          // An earlier kernel on this device failed: looked up once the first
+          // copies are on their way.
+          if (it == C::STAGES && *reinterpret_cast<volatile int*>(a.err) != 0) abort_flag = 1;
+          if (!mbar_wait(&bar_done[s], ((it / C::STAGES) & 1) ^ 1, a.err, kErrWaitEmpty, &abort_flag)) {
             ok = false;
             break;
           }
@@ -169,128 +284,165 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       for (uint32_t j = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; j < it; ++j)
         drain(&bar_full[j % C::STAGES], (j / C::STAGES) & 1, a.err);
     }
-  } else if (warp == 1) {
-    if (lane == 0) {
+    if (warp == 1) {
+      // bar_done of a stage tells both that the stage is free and that the
+      // block's sums are complete.
       constexpr uint32_t idesc = idesc_e4m3_f32(C::BM, C::BN);
       const uint64_t dbase = desc_k_sw128(smem_u32(smem));
+      const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+      const long total = (long)mine * kblocks;
       uint32_t it = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
-          const int s = it % C::STAGES;
-          const uint32_t b = it & 1;
-          if (!mbar_wait(&bar_acce[b], ((it >> 1) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag) ||
-              !mbar_wait(&bar_full[s], (it / C::STAGES) & 1, a.err, kErrWaitFull, &abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t da = desc_add(dbase, s * C::STAGE_BYTES), db = desc_add(da, C::A_BYTES);
-          const uint32_t d = tmem_base + b * C::BN;
-          mma_fp8_ss<false>(d, da, db, idesc);
-#pragma unroll
-          for (int k = 1; k < 4; ++k) mma_fp8_ss<true>(d, desc_add(da, k * 32), desc_add(db, k * 32), idesc);
-          mma_commit(&bar_empty[s]);
-          mma_commit(&bar_accf[b]);
-        }
+      bool full = false, free = true;  // tested ahead
+      for (; it < total; ++it) {
+        const int s = it % C::STAGES;
+        const uint32_t b = it & 1;
+        const uint64_t da = desc_add(dbase, s * C::STAGE_BYTES);
+        if (!warp_wait(full, &bar_full[s], (it / C::STAGES) & 1, a.err, kErrWaitFull, &abort_flag) ||
+            !warp_wait(free, &bar_acce[b], ((it >> 1) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag))
+          break;
+        tc_fence_after();
+        mma_block(tmem_base + b * C::BN, da, desc_add(da, C::A_BYTES), idesc, &bar_done[s]);
+        full = mbar_test(&bar_full[(it + 1) % C::STAGES], ((it + 1) / C::STAGES) & 1);
+        free = mbar_test(&bar_acce[b ^ 1], (((it + 1) >> 1) & 1) ^ 1);
       }
-      // The last stage-release commits land before the CTA can exit.
-      if (ok && !abort_flag)
+      // The last arrivals land before the CTA can exit.
+      if (it == total)
         for (uint32_t j = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; j < it; ++j)
-          if (!mbar_wait(&bar_empty[j % C::STAGES], (j / C::STAGES) & 1, a.err, kErrWaitDrain, &abort_flag)) break;
+          if (!warp_wait(&bar_done[j % C::STAGES], (j / C::STAGES) & 1, a.err, kErrWaitDrain, &abort_flag)) break;
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // Epilogue: warp w holds TMEM lanes 32 (w % 4) .. + 31, one row of x per
-    // thread, and one half (one output block) of the tile's columns.
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    uint4* stage = reinterpret_cast<uint4*>(smem + C::STAGES * C::STAGE_BYTES + (warp - 2) * C::EPI_STAGE);
-    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + half * 128;
+    // thread, and a quarter of the tile's columns.
+    const int q = warp & 3, quarter = (warp - 4) >> 2;
+    uint8_t* stage = smem + C::STAGES * C::STAGE_BYTES + (warp - 4) * C::EPI_STAGE;
+    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + quarter * C::COLS;
     uint32_t it = 0;
-    bool ok = true;
+    bool ok = true, done = false;  // done: the next block's barrier, tested ahead
     for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
       int mb, nb;
       tile_of(tile, tiles_m, tiles_n, mb, nb);
       const long row0 = (long)mb * C::BM + 32 * q;
       const float* sx = a.sx + min(row0 + lane, a.rows - 1);
-      const int ob = 2 * nb + half;
+      const int col0 = nb * C::BN + quarter * C::COLS, ob = col0 / kFp8Block;
       const float* sw = a.sw + (long)min(ob, oblocks - 1) * kblocks;
-      float acc[128];
+      uint64_t acc[C::COLS / 2];  // column pairs
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
-      float s_next = __ldg(sx) * __ldg(sw);
-      for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const float s = s_next;
-        if (kb + 1 < kblocks) s_next = __ldg(sx + (long)(kb + 1) * a.lds) * __ldg(sw + kb + 1);
-        const uint32_t b = it & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar_accf[b], (it >> 1) & 1, a.err, kErrWaitAccFull, &abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t r[2][16];
-        tmem_ld16(tm + b * C::BN, r[0]);
+      for (int i = 0; i < C::COLS / 2; ++i) acc[i] = 0;
+      if (a.bias) {  // padded with zeros to whole tiles
+        const ulonglong2* bp = reinterpret_cast<const ulonglong2*>(a.bias + col0);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          tmem_wait16(r[c & 1]);
-          if (c < 7) {
-            tmem_ld16(tm + b * C::BN + 16 * (c + 1), r[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar_acce[b]);
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(__uint_as_float(r[c & 1][i]), s, acc[16 * c + i]);
+        for (int i = 0; i < C::COLS / 4; ++i) {
+          const ulonglong2 b2 = __ldg(bp + i);
+          acc[2 * i] = b2.x;
+          acc[2 * i + 1] = b2.y;
         }
       }
-      if (!ok) break;
-      const int col0 = ob * 128;
-      if (col0 >= a.out) continue;
-      const int nrows = (int)min(32l, a.rows - row0);
-      if (a.bias) {
+      // The scales of two blocks are in hand, those of the next two on their
+      // way (a load is about two blocks' time away).
+      float x0 = __ldg(sx), x1 = __ldg(sx + (long)min(1, kblocks - 1) * a.lds), x2, x3;
+      float w0 = __ldg(sw), w1 = __ldg(sw + min(1, kblocks - 1)), w2, w3;
+      auto fetch = [&](int kb) {
+        const int k2 = min(kb, kblocks - 1), k3 = min(kb + 1, kblocks - 1);
+        x2 = __ldg(sx + (long)k2 * a.lds);
+        x3 = __ldg(sx + (long)k3 * a.lds);
+        w2 = __ldg(sw + k2);
+        w3 = __ldg(sw + k3);
+      };
+      fetch(2);
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const float s = (kb & 1) ? x1 * w1 : x0 * w0;
+        if (kb & 1) {
+          x0 = x2, x1 = x3, w0 = w2, w1 = w3;
+          fetch(kb + 3);
+        }
+        const uint64_t ss = pack_f32x2(s, s);
+        const uint32_t b = it & 1, src = tm + b * C::BN;
+        ok = warp_wait(done, &bar_done[it % C::STAGES], (it / C::STAGES) & 1, a.err, kErrWaitAccFull, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        // 16 columns at a time through two register blocks: the buffer goes
+        // back to the MMA issuer once the last block is loaded, with half of
+        // the sums still to be added.
+        uint32_t r[2][16];
+        auto add = [&](int c) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (col0 + i < a.out) acc[i] += __ldg(a.bias + col0 + i);
+          for (int i = 0; i < 8; ++i) fma_f32x2(acc[8 * c + i], pack_u32x2(r[c & 1][2 * i], r[c & 1][2 * i + 1]), ss);
+        };
+        tmem_ld16(src, r[0]);
+        tmem_ld16(src + 16, r[1]);
+        tmem_wait32(r);
+        add(0);
+        tmem_ld16(src + 32, r[0]);
+        add(1);
+        tmem_ld16(src + 48, r[1]);
+        tmem_wait32(r);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_acce[b]);
+        done = mbar_test(&bar_done[(it + 1) % C::STAGES], ((it + 1) / C::STAGES) & 1);
+        add(2);
+        add(3);
       }
-      if (nrows <= 0) continue;
-      if (a.y_vec && col0 + 128 <= a.out) {
-        const int size = a.y_dtype == G4M_F32 ? 4 : 2;
-        char* y = static_cast<char*>(a.y) + (row0 * a.ldy + col0) * size;
-        const size_t stride = (size_t)a.ldy * size;
+      if (!ok) break;
+      const int nrows = (int)min(32l, a.rows - row0);
+      if (nrows <= 0 || col0 >= a.out) continue;
+      float v[C::COLS];
+#pragma unroll
+      for (int i = 0; i < C::COLS / 2; ++i) unpack_f32x2(acc[i], v[2 * i], v[2 * i + 1]);
+      if (a.y_vec) {
+        // 64 bytes of each of the warp's 32 rows at a time, through shared
+        // memory (64-byte swizzle: 16-byte chunk c of row r at c ^ (r / 2 & 3))
+        // and out by TMA while the next tile's blocks are summed.
+        auto send = [&](const uint4 (&o)[4], int col) {
+          if (lane == 0) tma_store_read_wait();
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = o[i];
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tma_store_2d(&my, stage, col, (int)row0);
+        };
         if (a.y_dtype == G4M_F32) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint4 v[8];
+          for (int c = 0; c < C::COLS / 16; ++c) {
+            if (col0 + 16 * c >= a.out) break;
+            uint4 o[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              v[i] = make_uint4(__float_as_uint(acc[32 * c + 4 * i]), __float_as_uint(acc[32 * c + 4 * i + 1]),
-                                __float_as_uint(acc[32 * c + 4 * i + 2]), __float_as_uint(acc[32 * c + 4 * i + 3]));
-            warp_store_block<128>(stage, v, y + c * 128, stride, nrows, lane);
+            for (int i = 0; i < 4; ++i)
+              o[i] = make_uint4(__float_as_uint(v[16 * c + 4 * i]), __float_as_uint(v[16 * c + 4 * i + 1]),
+                                __float_as_uint(v[16 * c + 4 * i + 2]), __float_as_uint(v[16 * c + 4 * i + 3]));
+            send(o, col0 + 16 * c);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint4 v[8];
+          for (int c = 0; c < C::COLS / 32; ++c) {
+            if (col0 + 32 * c >= a.out) break;
+            uint4 o[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4; ++i) {
               uint32_t w[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float f0 = acc[64 * c + 8 * i + 2 * j], f1 = acc[64 * c + 8 * i + 2 * j + 1];
+                const float f0 = v[32 * c + 8 * i + 2 * j], f1 = v[32 * c + 8 * i + 2 * j + 1];
                 w[j] = a.y_dtype == G4M_BF16 ? pack2(f0, f1, __nv_bfloat16()) : pack2(f0, f1, __half());
               }
-              v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+              o[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            warp_store_block<128>(stage, v, y + c * 128, stride, nrows, lane);
+            send(o, col0 + 32 * c);
           }
         }
       } else if (lane < nrows) {
         with_type(a.y_dtype, [&](auto* tp) {
           auto* y = static_cast<decltype(tp)>(a.y) + (row0 + lane) * a.ldy + col0;
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (col0 + i < a.out) from_f32(acc[i], y + i);
+          for (int i = 0; i < C::COLS; ++i)
+            if (col0 + i < a.out) from_f32(v[i], y + i);
         });
       }
     }
+    if (lane == 0) tma_store_wait();
   }
 
   __syncthreads();
@@ -307,14 +459,21 @@ template <int NT>
 struct FewCfg {
   static constexpr int W_BYTES = kFp8TileBytes, X_BYTES = NT * 128;
   static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
-  static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 6;
+  static constexpr int STAGES = NT == 16 ? 5 : NT == 64 ? 3 : 4;
   static constexpr int BUFS = NT == 16 ? 8 : NT == 32 ? 8 : NT == 64 ? 4 : 2;  // accumulators in flight
   static constexpr int TMEM_COLS = BUFS * NT;
-  static constexpr int THREADS = 64 + 128;
+  // An epilogue warp holds 32 outputs of up to 32 rows: one warpgroup for each
+  // 32 rows (with 64 rows in a warp, a block's sums took 925 cycles).
+  static constexpr int RP = NT < 32 ? NT : 32, GROUPS = NT / RP;
+  static constexpr int SCALE_BLOCKS = NT == 16 ? 8 : NT == 32 ? 4 : 2;  // column blocks whose row scales are fetched together
+  static constexpr int SCALE_BYTES = 4 * 2 * SCALE_BLOCKS * NT * 4;     // per epilogue warp, double-buffered
+  static constexpr int PART_BYTES = NT * 128 * 4;  // partial totals from the cluster: splits * ceil(rows / splits) <= NT rows, splits a power of 2
+  static constexpr int BARS = 2 * STAGES + 2 * BUFS + 1;
+  static constexpr int THREADS = 64 + 128 * GROUPS;
   static constexpr int CTAS = NT <= 64 ? 2 : 1;  // per SM
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;
-  static_assert(NT * 128 * 4 <= STAGES * STAGE_BYTES, "the partial totals reuse the stages");
-  static_assert(CTAS * TMEM_COLS <= 512 && CTAS * (SMEM + 32 * NT + 2048) <= 233472, "over the SM's memories");
+  static constexpr int SMEM = STAGES * STAGE_BYTES + SCALE_BYTES + PART_BYTES + 1024;
+  static_assert(NT * 512 <= STAGES * STAGE_BYTES, "the outgoing totals reuse the stages");
+  static_assert(CTAS * TMEM_COLS <= 512 && CTAS * (SMEM + 1024 + 512) <= 233472, "over the SM's memories");
 };
 
 template <int NT>
@@ -322,8 +481,7 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, FewCfg<NT>::CTAS)
     fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ Fp8GemmArgs a, int splits) {
   using C = FewCfg<NT>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[C::STAGES], bar_empty[C::STAGES], bar_accf[C::BUFS], bar_acce[C::BUFS];
-  __shared__ __align__(16) float sc[4][2][NT];  // per epilogue warp: scale products of a block, double-buffered
+  __shared__ __align__(8) uint64_t bars[C::BARS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -334,40 +492,40 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, FewCfg<NT>::CTAS)
   const long row0 = (long)blockIdx.y * NT;
   const int nrows = (int)min((long)NT, a.rows - row0);
   const int k0 = (int)((long)kblocks * rank / splits), nk = (int)((long)kblocks * (rank + 1) / splits) - k0;
+  // The rows that this CTA of the cluster completes.
+  const int j0 = nrows * rank / splits, j1 = nrows * (rank + 1) / splits;
+  float* part = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES);
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&bar_full[s], 1);
-      mbar_init(&bar_empty[s], 1);
-    }
-    for (int b = 0; b < C::BUFS; ++b) {
-      mbar_init(&bar_accf[b], 1);
-      mbar_init(&bar_acce[b], 4);
-    }
-    // An earlier kernel on this device failed: nothing is waited for, but the
-    // CTA still meets its cluster's barriers.
-    abort_flag = *reinterpret_cast<volatile int*>(a.err) != 0;
+  uint64_t *bar_full = bars, *bar_empty = bars + C::STAGES, *bar_accf = bars + 2 * C::STAGES, *bar_acce = bar_accf + C::BUFS,
+           *bar_part = bars + C::BARS - 1;
+  if (threadIdx.x < C::BARS) {
+    mbar_init(bars + threadIdx.x, bars + threadIdx.x >= bar_acce && bars + threadIdx.x < bar_part ? 4 * C::GROUPS : 1);
     fence_mbar_init();
-    prefetch_tmap(&mx);
+    if (splits > 1 && bars + threadIdx.x == bar_part) mbar_expect_tx(bar_part, (uint32_t)(splits * (j1 - j0) * 512));
+    if (threadIdx.x == 0) abort_flag = 0;
   }
+  if (warp == 0 && lane == 0) prefetch_tmap(&mx);
   if (warp == 1) tmem_alloc(&tmem_slot, C::TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (splits > 1) cluster_arrive();  // this CTA's barriers can be reached from the others
   const uint32_t tmem_base = tmem_slot;
-  const bool run = abort_flag == 0;
-  __syncthreads();  // every thread has read the flag before a wait can raise it
-  const int q = warp & 3, t = 32 * q + lane;  // epilogue: output ob * 128 + t
-  float acc[NT];
+  // Epilogue: output ob * 128 + t, rows r0 .. r0 + RP - 1 of the tile.
+  const int q = warp & 3, t = 32 * q + lane, group = (warp - 2) >> 2, r0 = group * C::RP;
+  uint64_t acc[C::RP / 2];  // row pairs
 #pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = 0.0f;
+  for (int i = 0; i < C::RP / 2; ++i) acc[i] = 0;
 
   if (warp == 0) {
-    if (lane == 0 && run) {
+    if (lane == 0) {
       int it = 0;
       const uint8_t* w = a.w + ((long)ob * kblocks + k0) * kFp8TileBytes;
       for (; it < nk; ++it) {
         const int s = it % C::STAGES;
+        // An earlier kernel on this device failed: looked up once the first
+        // copies are on their way.
+        if (it == C::STAGES && *reinterpret_cast<volatile int*>(a.err) != 0) abort_flag = 1;
         if (!mbar_wait(&bar_empty[s], ((it / C::STAGES) & 1) ^ 1, a.err, kErrWaitEmpty, &abort_flag)) break;
         uint8_t* sw = smem + s * C::STAGE_BYTES;
         mbar_expect_tx(&bar_full[s], C::STAGE_BYTES);
@@ -378,114 +536,139 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, FewCfg<NT>::CTAS)
         drain(&bar_full[j % C::STAGES], (j / C::STAGES) & 1, a.err);
     }
   } else if (warp == 1) {
-    if (lane == 0 && run) {
-      constexpr uint32_t idesc = idesc_e4m3_f32(128, NT);
-      const uint64_t dbase = desc_k_sw128(smem_u32(smem));
-      int it = 0;
-      for (; it < nk; ++it) {
-        const int s = it % C::STAGES, b = it % C::BUFS;
-        if (!mbar_wait(&bar_acce[b], ((it / C::BUFS) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag) ||
-            !mbar_wait(&bar_full[s], (it / C::STAGES) & 1, a.err, kErrWaitFull, &abort_flag))
-          break;
-        tc_fence_after();
-        const uint64_t dw = desc_add(dbase, s * C::STAGE_BYTES), dx = desc_add(dw, C::W_BYTES);
-        const uint32_t d = tmem_base + b * NT;
-        mma_fp8_ss<false>(d, dw, dx, idesc);
-#pragma unroll
-        for (int k = 1; k < 4; ++k) mma_fp8_ss<true>(d, desc_add(dw, k * 32), desc_add(dx, k * 32), idesc);
-        mma_commit(&bar_empty[s]);
-        mma_commit(&bar_accf[b]);
-      }
-      if (it == nk)  // the last stage-release commits land before the stages are reused or the CTA exits
-        for (int j = it > C::STAGES ? it - C::STAGES : 0; j < it; ++j)
-          if (!mbar_wait(&bar_empty[j % C::STAGES], (j / C::STAGES) & 1, a.err, kErrWaitDrain, &abort_flag)) break;
+    constexpr uint32_t idesc = idesc_e4m3_f32(128, NT);
+    const uint64_t dbase = desc_k_sw128(smem_u32(smem));
+    int it = 0;
+    for (; it < nk; ++it) {
+      const int s = it % C::STAGES, b = it % C::BUFS;
+      const uint64_t dw = desc_add(dbase, s * C::STAGE_BYTES);
+      if (!warp_wait(&bar_acce[b], ((it / C::BUFS) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag) ||
+          !warp_wait(&bar_full[s], (it / C::STAGES) & 1, a.err, kErrWaitFull, &abort_flag))
+        break;
+      tc_fence_after();
+      mma_block(tmem_base + b * NT, dw, desc_add(dw, C::W_BYTES), idesc, &bar_accf[b]);
+      mma_commit_elected(&bar_empty[s]);
     }
-  } else if (run) {
-    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16);
+    if (it == nk)  // the last stage-release arrivals land before the CTA can exit
+      for (int j = it > C::STAGES ? it - C::STAGES : 0; j < it; ++j)
+        if (!warp_wait(&bar_empty[j % C::STAGES], (j / C::STAGES) & 1, a.err, kErrWaitDrain, &abort_flag)) break;
+  } else {
+    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + r0;
     const float* swp = a.sw + (long)ob * kblocks + k0;
     const float* sxp = a.sx + (long)k0 * a.lds + row0;
-    constexpr int PER = (NT + 31) / 32;
-    float nxt[PER];
-    auto fetch = [&](int i) {
+    // Row scales come a few column blocks at a time, one fetch ahead; the
+    // weight scales of 32 blocks sit in the lanes.
+    constexpr int SB = C::SCALE_BLOCKS;
+    float* sc = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + C::PART_BYTES) + (warp - 2) * 2 * SB * C::RP;
+    auto fetch = [&](int g) {
 #pragma unroll
-      for (int p = 0; p < PER; ++p) {
-        const int j = lane + 32 * p;
-        nxt[p] = i < nk && j < nrows ? __ldg(sxp + (long)i * a.lds + j) * __ldg(swp + i) : 0.0f;
+      for (int p = 0; p < SB * C::RP / 32; ++p) {
+        const int e = lane + 32 * p, i = g * SB + e / C::RP, j = r0 + e % C::RP;
+        const bool valid = i < nk && j < nrows;
+        cp_async4(sc + (g & 1) * SB * C::RP + e, valid ? sxp + (long)i * a.lds + j : sxp, valid);
       }
+      cp_async_commit();
     };
     fetch(0);
+    float wl = 0.0f, wn = lane < nk ? __ldg(swp + lane) : 0.0f;
     for (int i = 0; i < nk; ++i) {
-      float* s = sc[q][i & 1];
-#pragma unroll
-      for (int p = 0; p < PER; ++p)
-        if (lane + 32 * p < NT) s[lane + 32 * p] = nxt[p];
-      fetch(i + 1);
-      __syncwarp();
+      if ((i & 31) == 0) {
+        wl = wn;
+        wn = i + 32 + lane < nk ? __ldg(swp + i + 32 + lane) : 0.0f;
+      }
+      if (i % SB == 0) {
+        __syncwarp();  // every lane is done with the fetch before last
+        fetch(i / SB + 1);
+        cp_async_wait<1>();
+        __syncwarp();
+      }
+      const float w = __shfl_sync(0xffffffffu, wl, i & 31);
+      const uint64_t ww = pack_f32x2(w, w);
+      const float* s = sc + (i / SB & 1) * SB * C::RP + i % SB * C::RP;
       const int b = i % C::BUFS;
-      if (!__all_sync(0xffffffffu, mbar_wait(&bar_accf[b], (i / C::BUFS) & 1, a.err, kErrWaitAccFull, &abort_flag))) break;
+      if (!warp_wait(&bar_accf[b], (i / C::BUFS) & 1, a.err, kErrWaitAccFull, &abort_flag)) break;
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < NT / 16; ++c) {
+      for (int c = 0; c < C::RP / 16; ++c) {
         uint32_t r[16];
         tmem_ld16(tm + b * NT + 16 * c, r);
         tmem_wait16(r);
-        if (c == NT / 16 - 1) {
+        if (c == C::RP / 16 - 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_acce[b]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float4 f = *reinterpret_cast<const float4*>(s + 16 * c + 4 * j);
-          float* o = acc + 16 * c + 4 * j;
-          o[0] = fmaf(__uint_as_float(r[4 * j]), f.x, o[0]);
-          o[1] = fmaf(__uint_as_float(r[4 * j + 1]), f.y, o[1]);
-          o[2] = fmaf(__uint_as_float(r[4 * j + 2]), f.z, o[2]);
-          o[3] = fmaf(__uint_as_float(r[4 * j + 3]), f.w, o[3]);
+          const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(s + 16 * c + 4 * j);
+          fma_f32x2(acc[8 * c + 2 * j], pack_u32x2(r[4 * j], r[4 * j + 1]), mul_f32x2(f.x, ww));
+          fma_f32x2(acc[8 * c + 2 * j + 1], pack_u32x2(r[4 * j + 2], r[4 * j + 3]), mul_f32x2(f.y, ww));
         }
       }
     }
+    cp_async_wait<0>();
   }
 
   const int o = ob * 128 + t;
-  const float bias = warp >= 2 && o < a.out && a.bias ? __ldg(a.bias + o) : 0.0f;
+  const float bias = warp >= 2 && a.bias ? __ldg(a.bias + o) : 0.0f;  // padded with zeros to whole tiles
   if (splits == 1) {
     if (warp >= 2 && o < a.out)
       with_type(a.y_dtype, [&](auto* tp) {
-        auto* y = static_cast<decltype(tp)>(a.y) + row0 * a.ldy + o;
+        auto* y = static_cast<decltype(tp)>(a.y) + (row0 + r0) * a.ldy + o;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (j < nrows) from_f32(acc[j] + bias, y + j * a.ldy);
-      });
-  } else {
-    // Partial totals [row][128 outputs] replace the stages, whose copies and
-    // MMAs are done once every warp is here; each CTA of the cluster then
-    // adds a share of the rows in rank order.
-    __syncthreads();
-    float* part = reinterpret_cast<float*>(smem);
-    if (warp >= 2) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        if (j < nrows) part[j * 128 + t] = acc[j];
-    }
-    cluster_sync();
-    const int j0 = nrows * rank / splits, j1 = nrows * (rank + 1) / splits;
-    if (warp >= 2 && o < a.out)
-      with_type(a.y_dtype, [&](auto* tp) {
-        auto* y = static_cast<decltype(tp)>(a.y) + row0 * a.ldy + o;
-        for (int j = j0; j < j1; ++j) {
-          const uint32_t at = smem_u32(part + j * 128 + t);
-          float v[8];
-#pragma unroll
-          for (int p = 0; p < 8; ++p) v[p] = p < splits ? cluster_ld(at, p) : 0.0f;
-          float total = v[0];
-#pragma unroll
-          for (int p = 1; p < 8; ++p)
-            if (p < splits) total += v[p];
-          from_f32(total + bias, y + j * a.ldy);
+        for (int j = 0; j < C::RP; ++j) {
+          float v[2];
+          unpack_f32x2(acc[j / 2], v[0], v[1]);
+          if (r0 + j < nrows) from_f32(v[j & 1] + bias, y + j * a.ldy);
         }
       });
-    cluster_sync();  // no CTA leaves while its totals are being read
+  } else {
+    // Each CTA completes a share of the rows: all copy their partial totals of
+    // those rows ([row][128 outputs]) into its shared memory, and it adds them
+    // in rank order.  The stages hold the outgoing totals: their copies and
+    // MMAs are done.
+    bool ok = true;
+    if (warp >= 2) {
+      float* own = reinterpret_cast<float*>(smem) + r0 * 128 + t;
+#pragma unroll
+      for (int j = 0; j < C::RP; ++j) {
+        float v[2];
+        unpack_f32x2(acc[j / 2], v[0], v[1]);
+        if (r0 + j < nrows) own[j * 128] = v[j & 1];
+      }
+      fence_proxy_async_smem();
+      asm volatile("bar.sync 1, %0;" ::"n"(128 * C::GROUPS) : "memory");
+    }
+    cluster_wait();
+    if (warp >= 2) {
+      if (warp == 2 && lane < splits) {
+        const int begin = nrows * lane / splits, n = nrows * (lane + 1) / splits - begin;
+        if (n > 0)
+          cluster_push(cluster_map(smem_u32(part + rank * n * 128), lane), smem + begin * 512, n * 512,
+                       cluster_map(smem_u32(bar_part), lane));
+      }
+      __syncwarp();
+      ok = warp_wait(bar_part, 0, a.err, kErrWaitAccFull, &abort_flag);
+      if (ok && o < a.out)
+        with_type(a.y_dtype, [&](auto* tp) {
+          auto* y = static_cast<decltype(tp)>(a.y) + row0 * a.ldy + o;
+#pragma unroll 2
+          for (int j = j0 + group; j < j1; j += C::GROUPS) {
+            const float* from = part + (j - j0) * 128 + t;
+            float v[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) v[p] = p < splits ? from[p * (j1 - j0) * 128] : 0.0f;
+            float total = v[0];
+#pragma unroll
+            for (int p = 1; p < 8; ++p)
+              if (p < splits) total += v[p];
+            from_f32(total + bias, y + j * a.ldy);
+          }
+        });
+    }
+    // No CTA leaves while another one may still push to it.
+    cluster_arrive_relaxed();
+    cluster_wait();
   }
   __syncthreads();
   if (warp == 1) {
@@ -566,11 +749,13 @@ cudaError_t fp8_gemm(const Fp8GemmArgs& a, int dev, cudaStream_t st) {
   if (a.rows <= 32) return launch_few<32>(a, sms, st);
   if (a.rows <= 64) return launch_few<64>(a, sms, st);
   if (a.rows <= 256) return launch_few<128>(a, sms, st);
-  CUtensorMap mx;
+  CUtensorMap mx, my;
   if (!make_tmap_u8_pitch(&mx, a.x, a.rows, a.in, a.ldx, ManyCfg::BM)) return cudaErrorInvalidValue;
+  if (!a.y_vec) my = mx;  // not used
+  else if (!make_tmap_out(&my, a.y, a.rows, a.out, a.ldy, a.y_dtype == G4M_F32 ? 4 : 2, 32)) return cudaErrorInvalidValue;
   const long tiles = (a.rows + ManyCfg::BM - 1) / ManyCfg::BM * ((fp8_blocks(a.out) + 1) / 2);
   if (tiles > 0x3fffffffL) return cudaErrorInvalidValue;
-  fp8_gemm_many_kernel<<<(unsigned)std::min<long>(tiles, sms), ManyCfg::THREADS, ManyCfg::SMEM, st>>>(mx, a);
+  fp8_gemm_many_kernel<<<(unsigned)std::min<long>(tiles, sms), ManyCfg::THREADS, ManyCfg::SMEM, st>>>(mx, my, a);
   return cudaGetLastError();
 }
 

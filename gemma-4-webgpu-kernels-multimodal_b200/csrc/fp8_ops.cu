@@ -184,11 +184,16 @@ int g4m_fp8_linear_prepare(g4m_ctx* ctx, int di, const uint8_t* w, const float* 
     L->in = in;
     L->out = out;
     uint8_t* raw = nullptr;
+    std::vector<float> padded;
+    if (bias) {
+      padded.assign((size_t)(fp8_blocks(out) + 1) / 2 * 2 * kFp8Block, 0.0f);
+      memcpy(padded.data(), bias, (size_t)out * sizeof(float));
+    }
     const bool ok = fp8_gemm_setup() == cudaSuccess && to_device(&raw, w, (size_t)out * in) &&
                     cudaMalloc(&L->w, fp8_weight_bytes(out, in)) == cudaSuccess &&
                     fp8_weight_tiles(raw, out, in, L->w, cudaStreamLegacy) == cudaSuccess &&
                     to_device(&L->sw, w_scales, (size_t)(fp8_blocks(out) * fp8_blocks(in))) &&
-                    (!bias || to_device(&L->bias, bias, (size_t)out)) &&
+                    (!bias || to_device(&L->bias, padded.data(), padded.size())) &&
                     cudaStreamSynchronize(cudaStreamLegacy) == cudaSuccess;
     if (raw) cudaFree(raw);
     if (!ok) {

@@ -57,7 +57,7 @@ struct Fp8GemmArgs {
   long lds;
   const uint8_t* w;  // tiles
   const float* sw;   // [blocks of out][blocks of in]
-  const float* bias;
+  const float* bias; // [blocks of out, padded to an even number, x 128], zeros past out; or null
   void* y;
   int y_dtype, y_vec;  // y_vec: rows of y start on 16-byte boundaries
   long ldy;

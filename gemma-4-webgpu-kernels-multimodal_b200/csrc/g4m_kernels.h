@@ -97,6 +97,8 @@ bool make_tmap_f16_any(CUtensorMap* map, const void* base, uint64_t rows, uint64
                        uint32_t box_rows);
 bool make_tmap_u8_pitch(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch,
                         uint32_t box_rows);
+bool make_tmap_out(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems, int elem,
+                   uint32_t box_rows);
 int g_num_sms(int dev);
 
 cudaError_t prep_a(const float* x, long rows, int cols, float s_in, const float* row_scale, __half* hi, __half* lo,

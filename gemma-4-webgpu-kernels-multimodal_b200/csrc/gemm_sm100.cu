@@ -711,6 +711,23 @@ bool make_tmap_u8_pitch(CUtensorMap* map, const void* base, uint64_t rows, uint6
   return r == CUDA_SUCCESS;
 }
 
+// Output matrix of 4- or 2-byte elements [rows, cols] with a 16-byte-multiple
+// row pitch `pitch_elems`: box of 64 bytes x box_rows rows, 64B swizzle.
+bool make_tmap_out(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems, int elem,
+                   uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || !base || (pitch_elems * elem) % 16 != 0 || pitch_elems < cols || (reinterpret_cast<uintptr_t>(base) % 16) != 0)
+    return false;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch_elems * elem};
+  cuuint32_t box[2] = {64u / elem, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims,
+                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 int g_num_sms(int dev) {
   static int cache[64] = {0};
   if (dev < 0 || dev >= 64) return 148;
