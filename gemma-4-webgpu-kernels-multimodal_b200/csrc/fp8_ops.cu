@@ -146,7 +146,7 @@ int g4m_fp8_quantize(g4m_ctx* ctx, int di, int act, const void* x, int dtype, in
     Device& d = *ctx->devs[di];
     DeviceGuard guard(d.id);
     cudaStream_t st = stream_of(stream);
-    G4M_RUN("fp8_quantize", fp8_quantize(a, st));
+    G4M_RUN("fp8_quantize", fp8_quantize(a, d.id, st));
     return G4M_OK;
   });
 }
@@ -167,7 +167,7 @@ int g4m_norm_residual(g4m_ctx* ctx, int di, const g4m_norm_args* args, void* str
     Device& d = *ctx->devs[di];
     DeviceGuard guard(d.id);
     cudaStream_t st = stream_of(stream);
-    G4M_RUN("norm_residual", norm_residual(a, st));
+    G4M_RUN("norm_residual", norm_residual(a, d.id, st));
     return G4M_OK;
   });
 }
@@ -369,7 +369,7 @@ int g4m_rope_run(g4m_rope* R, const g4m_rope_view* q, const g4m_rope_view* k, in
     Device& d = *R->d;
     DeviceGuard guard(R->dev);
     cudaStream_t st = stream_of(stream);
-    G4M_RUN("rope", rope_run(a, st));
+    G4M_RUN("rope", rope_run(a, R->dev, st));
     return G4M_OK;
   });
 }

@@ -20,10 +20,10 @@ struct QuantArgs {
   float* scales;
   long lds;
 };
-cudaError_t fp8_quantize(const QuantArgs& a, cudaStream_t st);
+cudaError_t fp8_quantize(const QuantArgs& a, int dev, cudaStream_t st);
 
 constexpr int kNormMaxD = 16384;
-cudaError_t norm_residual(const g4m_norm_args& a, cudaStream_t st);
+cudaError_t norm_residual(const g4m_norm_args& a, int dev, cudaStream_t st);
 
 struct RopeArgs {
   const uint64_t* turns;  // [rotary / 2] turns per position, 0.64 fixed point
@@ -34,9 +34,8 @@ struct RopeArgs {
   int copy[2];            // elements from `rotary` on have to be copied
   long tokens;
   const void* positions;
-  int token_block, head_slices;  // filled in by the launcher
 };
-cudaError_t rope_run(RopeArgs a, cudaStream_t st);
+cudaError_t rope_run(const RopeArgs& a, int dev, cudaStream_t st);
 
 // Weights live in HBM as the tiles the tensor core reads: 128 outputs x 128
 // columns of codes, 16 KB each, in the 128-byte-swizzled order of shared

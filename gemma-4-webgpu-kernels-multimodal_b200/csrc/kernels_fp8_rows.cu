@@ -4,72 +4,92 @@
 #include <algorithm>
 
 #include "fp8_rows.cuh"
+#include "g4m_kernels.h"
 #include "g4m_sm100.cuh"
 
 namespace g4m {
 
 // ---------------------------------------------------------------------------
 // Quantiser.  16 lanes hold one block (8 columns each): the block's largest
-// magnitude is four shuffles, and nothing else crosses lanes.  Each half-warp
-// takes kQuantUnroll blocks, all of whose loads are issued before the first
-// is used.
+// magnitude is four shuffles, and nothing else crosses lanes.  Half-warps
+// walk the blocks of all rows with the next block's loads in flight.
 // ---------------------------------------------------------------------------
 constexpr int kQuantThreads = 256;
-constexpr int kQuantUnroll = 2;
 
+// act(x0) * x1.  The gate's sigmoid argument is scaled by -log2(e) in its
+// constants: x sigmoid(z) = x / (1 + 2^(-z log2 e)).
 template <int ACT>
 __device__ __forceinline__ float activate(float x0, float x1) {
-  if (ACT == G4M_ACT_SILU) return x0 * sigmoid_f(x0) * x1;
-  // gelu_tanh(x) = x sigmoid(2 u), u = sqrt(2/pi) (x + 0.044715 x^3)
-  const float u = 0.7978845608028654f * (x0 + 0.044715f * x0 * x0 * x0);
-  return x0 * sigmoid_f(2.0f * u) * x1;
+  float e;  // -z log2 e: z = x for silu, z = 2 sqrt(2/pi) (x + 0.044715 x^3) for gelu_tanh
+  if (ACT == G4M_ACT_SILU) {
+    e = x0 * -kLog2eF;
+  } else {
+    constexpr float k1 = -2.0f * 0.7978845608028654f * kLog2eF, k3 = k1 * 0.044715f;
+    e = x0 * fmaf(k3, x0 * x0, k1);
+  }
+  return x0 * rcp_approx(1.0f + ex2_approx(e)) * x1;
 }
 
-template <class T, int ACT>
-__global__ void __launch_bounds__(kQuantThreads) fp8_quantize_kernel(QuantArgs a) {
-  constexpr int PER = kQuantThreads / 16;
+template <class T, int ACT, bool FULL>
+__global__ void __launch_bounds__(kQuantThreads, 5) fp8_quantize_kernel(const __grid_constant__ QuantArgs a, FastDiv blocks) {
   const int lane16 = threadIdx.x & 15;
-  const uint32_t u0 = blockIdx.x * (PER * kQuantUnroll) + (threadIdx.x >> 4);
-  float v[kQuantUnroll][8], g[kQuantUnroll][8];
-  uint32_t row[kQuantUnroll], kb[kQuantUnroll];
-#pragma unroll
-  for (int i = 0; i < kQuantUnroll; ++i) {
-    const uint32_t u = u0 + i * PER;
-    row[i] = u / (uint32_t)a.blocks;
-    kb[i] = u - row[i] * (uint32_t)a.blocks;
-    const int c = (int)kb[i] * kFp8Block + lane16 * 8;
-    const int d = u < a.units ? a.d : 0;  // past the end: zeros, nothing read
-    const T* x = static_cast<const T*>(a.x) + (long)row[i] * a.ldx;
-    load8(x, c, d, a.vec & 1, v[i]);
-    if (ACT != G4M_ACT_NONE) load8(x + a.d, c, d, a.vec & 2, g[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < kQuantUnroll; ++i) {
+  const uint32_t stride = gridDim.x * (kQuantThreads / 16);
+  uint32_t u = blockIdx.x * (kQuantThreads / 16) + (threadIdx.x >> 4);
+  Raw8<T> x0, x1;
+  uint32_t row = 0, kb = 0;
+  auto fetch = [&](uint32_t unit) {
+    row = div_by(unit, blocks);
+    kb = unit - row * blocks.d;
+    const int c = (int)kb * kFp8Block + lane16 * 8;
+    const int d = unit < a.units ? a.d : 0;  // past the end: zeros, nothing read
+    const T* x = static_cast<const T*>(a.x) + (long)row * a.ldx;
+    load_raw8<FULL>(x, c, d, a.vec & 1, x0);
+    if (ACT != G4M_ACT_NONE) load_raw8<FULL>(x + a.d, c, d, a.vec & 2, x1);
+  };
+  fetch(u);
+  // The two half-warps of a warp hold neighbouring blocks and stay together:
+  // the warp goes on while its first has a block.
+  for (; u - ((threadIdx.x >> 4) & 1) < a.units; u += stride) {
+    float v[8];
+    unpack8(x0, v);
     if (ACT != G4M_ACT_NONE) {
+      float g[8];
+      unpack8(x1, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = activate<ACT>(v[i][j], g[i][j]);
+      for (int j = 0; j < 8; ++j) v[j] = activate<ACT>(v[j], g[j]);
     }
-    const float s = fp8_scale(block_amax_bits(amax_bits8(v[i])));
-    if (u0 + i * PER < a.units) {
-      store_codes8(a.codes + (long)row[i] * a.ldc, (int)kb[i] * kFp8Block + lane16 * 8, a.d, fp8_encode8(v[i], s));
-      if (lane16 == 0) a.scales[(long)kb[i] * a.lds + row[i]] = s;
+    const uint32_t r = row, k = kb;
+    fetch(u + stride);
+    const float s = fp8_scale(block_amax_bits(amax_bits8(v)));
+    if (u < a.units) {
+      store_codes8<FULL>(a.codes + (long)r * a.ldc, (int)k * kFp8Block + lane16 * 8, a.d, fp8_encode8(v, s));
+      if (lane16 == 0) a.scales[(long)k * a.lds + r] = s;
     }
   }
 }
 
 template <class T>
-static void launch_quantize(const QuantArgs& a, cudaStream_t st) {
-  constexpr uint32_t per = kQuantThreads / 16 * kQuantUnroll;
-  const uint32_t grid = (a.units - 1) / per + 1;
-  if (a.act == G4M_ACT_SILU) fp8_quantize_kernel<T, G4M_ACT_SILU><<<grid, kQuantThreads, 0, st>>>(a);
-  else if (a.act == G4M_ACT_GELU_TANH) fp8_quantize_kernel<T, G4M_ACT_GELU_TANH><<<grid, kQuantThreads, 0, st>>>(a);
-  else fp8_quantize_kernel<T, G4M_ACT_NONE><<<grid, kQuantThreads, 0, st>>>(a);
+static void launch_quantize(const QuantArgs& a, int sms, cudaStream_t st) {
+  const uint32_t per = kQuantThreads / 16, all = (a.units - 1) / per + 1;
+  const uint32_t grid = std::min<uint32_t>(all, (uint32_t)sms * 5);
+  const FastDiv blocks = fast_div((uint32_t)a.blocks);
+  auto go = [&](auto kernel) { kernel<<<grid, kQuantThreads, 0, st>>>(a, blocks); };
+  if (a.d % 8 == 0 && (a.vec & 1) && (a.act == G4M_ACT_NONE || (a.vec & 2))) {
+    if (a.act == G4M_ACT_SILU) go(fp8_quantize_kernel<T, G4M_ACT_SILU, true>);
+    else if (a.act == G4M_ACT_GELU_TANH) go(fp8_quantize_kernel<T, G4M_ACT_GELU_TANH, true>);
+    else go(fp8_quantize_kernel<T, G4M_ACT_NONE, true>);
+  } else {
+    if (a.act == G4M_ACT_SILU) go(fp8_quantize_kernel<T, G4M_ACT_SILU, false>);
+    else if (a.act == G4M_ACT_GELU_TANH) go(fp8_quantize_kernel<T, G4M_ACT_GELU_TANH, false>);
+    else go(fp8_quantize_kernel<T, G4M_ACT_NONE, false>);
+  }
 }
 
-cudaError_t fp8_quantize(const QuantArgs& a, cudaStream_t st) {
-  if (a.dtype == G4M_F32) launch_quantize<float>(a, st);
-  else if (a.dtype == G4M_BF16) launch_quantize<__nv_bfloat16>(a, st);
-  else launch_quantize<__half>(a, st);
+cudaError_t fp8_quantize(const QuantArgs& a, int dev, cudaStream_t st) {
+  const int sms = g_num_sms(dev);
+  if (a.dtype == G4M_F32) launch_quantize<float>(a, sms, st);
+  else if (a.dtype == G4M_BF16) launch_quantize<__nv_bfloat16>(a, sms, st);
+  else launch_quantize<__half>(a, sms, st);
   return cudaGetLastError();
 }
 
@@ -78,15 +98,20 @@ cudaError_t fp8_quantize(const QuantArgs& a, cudaStream_t st) {
 // thread t of the row's T threads holds columns [8 (k T + t), + 8) for
 // k < NCH, so 16 consecutive lanes hold one 128-column block and the e4m3
 // scales need no shared memory.  The two means of squares are the only row
-// sums.
+// sums.  Blocks walk the rows with the next row's loads in flight: with one
+// row per block, loads, sums and stores took turns.
 // ---------------------------------------------------------------------------
 struct NormKernelArgs {
   g4m_norm_args a;
   uint32_t vec;  // which row sets start on 16-byte boundaries (bits below)
+  float inv_d;
+  FastDiv per_gate;
 };
 enum : uint32_t { kVecY = 1, kVecGate = 2, kVecH = 4, kVecHOut = 8, kVecN = 16, kVecPost = 32, kVecPre = 64 };
 
-// Sum over the threads of the row; every thread gets it.
+// Sum over the threads of the row; every thread gets it.  The two sums of a
+// row alternate between two `part`s, so that one barrier each is enough: a
+// part is written again only after the other sum's barrier.
 __device__ __forceinline__ float row_sum(float v, float* part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -111,10 +136,11 @@ __device__ __forceinline__ float square_sum(const float (&v)[NCH][8]) {
 }
 
 // v = v * inv * w for the chunk at column c (w null: all ones).
+template <bool FULL>
 __device__ __forceinline__ void scale8(float (&v)[8], float inv, const float* w, int c, int d, bool vec) {
   if (w) {
     float f[8];
-    load8(w, c, d, vec, f);
+    load8<FULL>(w, c, d, vec, f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (v[i] * inv) * f[i];
   } else {
@@ -123,78 +149,90 @@ __device__ __forceinline__ void scale8(float (&v)[8], float inv, const float* w,
   }
 }
 
+// Chunks per thread, the most threads of a row, blocks an SM shall hold.
 template <int NCH>
-__global__ void __launch_bounds__(512) norm_residual_kernel(const __grid_constant__ NormKernelArgs p) {
+struct NormCfg {
+  static constexpr int T = NCH == 4 ? 512 : 256;
+  static constexpr int BLOCKS = NCH == 1 ? 4 : NCH == 2 ? 3 : 1;
+};
+
+template <class TY, class TH, int NCH, bool FULL>
+__global__ void __launch_bounds__(NormCfg<NCH>::T, NormCfg<NCH>::BLOCKS)
+    norm_residual_kernel(const __grid_constant__ NormKernelArgs p) {
   __shared__ float part[2][16];
   const g4m_norm_args& a = p.a;
   const int T = blockDim.x, t = threadIdx.x, d = a.d;
-  const long row = blockIdx.x;
-  float b[NCH][8], h[NCH][8];
+  Raw8<TY> ry[NCH];
+  Raw8<TH> rh[NCH];
+  auto fetch = [&](long row) {
+    const int dd = row < a.rows ? d : 0;  // past the end: zeros, nothing read
+    const TY* y = static_cast<const TY*>(a.y) + row * a.ldy;
+    const TH* x = static_cast<const TH*>(a.h) + row * a.ldh;
 #pragma unroll
-  for (int k = 0; k < NCH; ++k)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[k][i] = h[k][i] = 0.0f;
-  if (a.y)
-    with_type(a.dtype, [&](auto* tp) {
-      auto* y = static_cast<decltype(tp)>(const_cast<void*>(a.y)) + row * a.ldy;
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) load8(y, 8 * (k * T + t), d, p.vec & kVecY, b[k]);
-    });
-  if (a.h)
-    with_type(a.h_dtype, [&](auto* tp) {
-      auto* x = static_cast<decltype(tp)>(const_cast<void*>(a.h)) + row * a.ldh;
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) load8(x, 8 * (k * T + t), d, p.vec & kVecH, h[k]);
-    });
-  if (a.y) {
-    if (a.norm_post) {
-      const float inv = 1.0f / sqrtf(row_sum(square_sum<NCH>(b), part[0]) / (float)d + a.eps);
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) scale8(b[k], inv, a.w_post, 8 * (k * T + t), d, p.vec & kVecPost);
+    for (int k = 0; k < NCH; ++k) {
+      load_raw8<FULL>(y, 8 * (k * T + t), a.y ? dd : 0, p.vec & kVecY, ry[k]);
+      load_raw8<FULL>(x, 8 * (k * T + t), a.h ? dd : 0, p.vec & kVecH, rh[k]);
     }
-    if (a.gate)
-      with_type(a.dtype, [&](auto* tp) {
-        auto* g = static_cast<decltype(tp)>(const_cast<void*>(a.gate)) + row / a.rows_per_gate * a.ldg;
+  };
+  // Rows of one warp share a block four at a time and meet no block barrier.
+  const long stride = (long)gridDim.x * blockDim.y;
+  long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
+  fetch(row);
+  for (; row < a.rows; row += stride) {
+    float b[NCH][8], h[NCH][8];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      unpack8(ry[k], b[k]);
+      unpack8(rh[k], h[k]);
+    }
+    fetch(row + stride);
+    if (a.y) {
+      if (a.norm_post) {
+        const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(b), part[0]), p.inv_d, a.eps));
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) scale8<FULL>(b[k], inv, a.w_post, 8 * (k * T + t), d, p.vec & kVecPost);
+      }
+      if (a.gate) {
+        const TY* g = static_cast<const TY*>(a.gate) + (long)div_by((uint32_t)row, p.per_gate) * a.ldg;
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
           float f[8];
-          load8(g, 8 * (k * T + t), d, p.vec & kVecGate, f);
+          load8<FULL>(g, 8 * (k * T + t), d, p.vec & kVecGate, f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) b[k][i] *= f[i];
         }
-      });
-  }
+      }
+    }
 #pragma unroll
-  for (int k = 0; k < NCH; ++k)
+    for (int k = 0; k < NCH; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[k][i] = a.res_scale * fmaf(a.branch_scale, b[k][i], h[k][i]);
-  if (a.h_out)
-    with_type(a.h_dtype, [&](auto* tp) {
-      auto* o = static_cast<decltype(tp)>(a.h_out) + row * a.ldh_out;
+      for (int i = 0; i < 8; ++i) h[k][i] = a.res_scale * fmaf(a.branch_scale, b[k][i], h[k][i]);
+    if (a.h_out) {
+      TH* o = static_cast<TH*>(a.h_out) + row * a.ldh_out;
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) store8(o, 8 * (k * T + t), d, p.vec & kVecHOut, h[k]);
-    });
-  if (!a.n_out && !a.out.codes) return;
-  if (a.norm_pre) {
-    const float inv = 1.0f / sqrtf(row_sum(square_sum<NCH>(h), part[1]) / (float)d + a.eps);
+      for (int k = 0; k < NCH; ++k) store8<FULL>(o, 8 * (k * T + t), d, p.vec & kVecHOut, h[k]);
+    }
+    if (!a.n_out && !a.out.codes) continue;
+    if (a.norm_pre) {
+      const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(h), part[1]), p.inv_d, a.eps));
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) scale8(h[k], inv, a.w_pre, 8 * (k * T + t), d, p.vec & kVecPre);
-  }
-  if (a.n_out)
-    with_type(a.dtype, [&](auto* tp) {
-      auto* o = static_cast<decltype(tp)>(a.n_out) + row * a.ldn;
+      for (int k = 0; k < NCH; ++k) scale8<FULL>(h[k], inv, a.w_pre, 8 * (k * T + t), d, p.vec & kVecPre);
+    }
+    if (a.n_out) {
+      TY* o = static_cast<TY*>(a.n_out) + row * a.ldn;
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) store8(o, 8 * (k * T + t), d, p.vec & kVecN, h[k]);
-    });
-  if (a.out.codes) {
-    uint8_t* codes = a.out.codes + row * a.out.ldc;
+      for (int k = 0; k < NCH; ++k) store8<FULL>(o, 8 * (k * T + t), d, p.vec & kVecN, h[k]);
+    }
+    if (a.out.codes) {
+      uint8_t* codes = a.out.codes + row * a.out.ldc;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      const int c = 8 * (k * T + t);
-      const float s = fp8_scale(block_amax_bits(amax_bits8(h[k])));
-      if (c < d) {
-        store_codes8(codes, c, d, fp8_encode8(h[k], s));
-        if ((t & 15) == 0) a.out.scales[(long)(c / kFp8Block) * a.out.lds + row] = s;
+      for (int k = 0; k < NCH; ++k) {
+        const int c = 8 * (k * T + t);
+        const float s = fp8_scale(block_amax_bits(amax_bits8(h[k])));
+        if (c < d) {
+          store_codes8<FULL>(codes, c, d, fp8_encode8(h[k], s));
+          if ((t & 15) == 0) a.out.scales[(long)(c / kFp8Block) * a.out.lds + row] = s;
+        }
       }
     }
   }
@@ -205,19 +243,46 @@ static bool rows16(const void* p, int64_t ld, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * size)) % 16 == 0;
 }
 
-cudaError_t norm_residual(const g4m_norm_args& a, cudaStream_t st) {
+template <class TY, class TH, int NCH>
+static void launch_norm(const NormKernelArgs& p, int sms, cudaStream_t st) {
+  const int chunks = (p.a.d + 7) / 8, T = ((chunks + NCH - 1) / NCH + 31) / 32 * 32;
+  const dim3 block(T, T == 32 ? 4 : 1);
+  const long blocks = (p.a.rows + block.y - 1) / block.y;
+  const long resident = (long)sms * std::max(1, NormCfg<NCH>::T * NormCfg<NCH>::BLOCKS / (T * (int)block.y));
+  const g4m_norm_args& a = p.a;
+  const bool full = a.d % 8 == 0 && (!a.y || (p.vec & kVecY)) && (!a.gate || (p.vec & kVecGate)) && (!a.h || (p.vec & kVecH)) &&
+                    (!a.h_out || (p.vec & kVecHOut)) && (!a.n_out || (p.vec & kVecN)) && (!a.w_post || (p.vec & kVecPost)) &&
+                    (!a.w_pre || (p.vec & kVecPre));
+  if (full) norm_residual_kernel<TY, TH, NCH, true><<<(unsigned)std::min(blocks, resident), block, 0, st>>>(p);
+  else norm_residual_kernel<TY, TH, NCH, false><<<(unsigned)std::min(blocks, resident), block, 0, st>>>(p);
+}
+template <class TY, class TH>
+static void launch_norm_h(const NormKernelArgs& p, int sms, cudaStream_t st) {
+  const int chunks = (p.a.d + 7) / 8;
+  if (chunks <= 256) launch_norm<TY, TH, 1>(p, sms, st);
+  else if (chunks <= 512) launch_norm<TY, TH, 2>(p, sms, st);
+  else launch_norm<TY, TH, 4>(p, sms, st);
+}
+template <class TY>
+static void launch_norm_y(const NormKernelArgs& p, int sms, cudaStream_t st) {
+  if (p.a.h_dtype == G4M_F32) launch_norm_h<TY, float>(p, sms, st);
+  else if (p.a.h_dtype == G4M_BF16) launch_norm_h<TY, __nv_bfloat16>(p, sms, st);
+  else launch_norm_h<TY, __half>(p, sms, st);
+}
+
+cudaError_t norm_residual(const g4m_norm_args& a, int dev, cudaStream_t st) {
   NormKernelArgs p;
   p.a = a;
   p.vec = (rows16(a.y, a.ldy, a.dtype) ? kVecY : 0) | (rows16(a.gate, a.ldg, a.dtype) ? kVecGate : 0) |
           (rows16(a.h, a.ldh, a.h_dtype) ? kVecH : 0) | (rows16(a.h_out, a.ldh_out, a.h_dtype) ? kVecHOut : 0) |
           (rows16(a.n_out, a.ldn, a.dtype) ? kVecN : 0) | (rows16(a.w_post, 0, G4M_F32) ? kVecPost : 0) |
           (rows16(a.w_pre, 0, G4M_F32) ? kVecPre : 0);
-  const int chunks = (a.d + 7) / 8;
-  const unsigned grid = (unsigned)a.rows;
-  auto threads = [&](int nch) { return std::max(32, ((chunks + nch - 1) / nch + 31) / 32 * 32); };
-  if (chunks <= 512) norm_residual_kernel<1><<<grid, threads(1), 0, st>>>(p);
-  else if (chunks <= 1024) norm_residual_kernel<2><<<grid, threads(2), 0, st>>>(p);
-  else norm_residual_kernel<4><<<grid, threads(4), 0, st>>>(p);
+  p.inv_d = 1.0f / (float)a.d;
+  p.per_gate = fast_div((uint32_t)std::min<int64_t>(std::max<int64_t>(a.rows_per_gate, 1), 0x7fffffff));
+  const int sms = g_num_sms(dev);
+  if (a.dtype == G4M_F32) launch_norm_y<float>(p, sms, st);
+  else if (a.dtype == G4M_BF16) launch_norm_y<__nv_bfloat16>(p, sms, st);
+  else launch_norm_y<__half>(p, sms, st);
   return cudaGetLastError();
 }
 
