@@ -111,33 +111,6 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[2][16]) {
   for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[1][i])::"memory");
 }
 
-// Pairs of f32 in one register pair: one instruction for two fma.  The f32
-// pipe takes two cycles for it, so the gain is in issue slots, which the
-// waiting warps need.
-__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  return v;
-}
-__device__ __forceinline__ uint64_t pack_u32x2(uint32_t a, uint32_t b) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
-  return v;
-}
-__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-// acc += x * s, elementwise, each rounded to nearest.
-__device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t x, uint64_t s) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(x), "l"(s));
-}
-
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
-  uint64_t v;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-  return v;
-}
-
 // A tile of this CTA's shared memory to global memory (the map's box and swizzle);
 // rows and columns past the tensor's edges are not written.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {

@@ -164,20 +164,23 @@ __global__ void __launch_bounds__(NormCfg<NCH>::T, NormCfg<NCH>::BLOCKS)
   const int T = blockDim.x, t = threadIdx.x, d = a.d;
   Raw8<TY> ry[NCH];
   Raw8<TH> rh[NCH];
-  auto fetch = [&](long row) {
-    const int dd = row < a.rows ? d : 0;  // past the end: zeros, nothing read
+  auto fetch_y = [&](long row) {
+    const int dd = row < a.rows && a.y ? d : 0;  // past the end: zeros, nothing read
     const TY* y = static_cast<const TY*>(a.y) + row * a.ldy;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) load_raw8<FULL>(y, 8 * (k * T + t), dd, p.vec & kVecY, ry[k]);
+  };
+  auto fetch_h = [&](long row) {
+    const int dd = row < a.rows && a.h ? d : 0;
     const TH* x = static_cast<const TH*>(a.h) + row * a.ldh;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      load_raw8<FULL>(y, 8 * (k * T + t), a.y ? dd : 0, p.vec & kVecY, ry[k]);
-      load_raw8<FULL>(x, 8 * (k * T + t), a.h ? dd : 0, p.vec & kVecH, rh[k]);
-    }
+    for (int k = 0; k < NCH; ++k) load_raw8<FULL>(x, 8 * (k * T + t), dd, p.vec & kVecH, rh[k]);
   };
   // Rows of one warp share a block four at a time and meet no block barrier.
   const long stride = (long)gridDim.x * blockDim.y;
   long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
-  fetch(row);
+  fetch_y(row);
+  fetch_h(row);
   for (; row < a.rows; row += stride) {
     float b[NCH][8], h[NCH][8];
 #pragma unroll
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(NormCfg<NCH>::T, NormCfg<NCH>::BLOCKS)
       unpack8(ry[k], b[k]);
       unpack8(rh[k], h[k]);
     }
-    fetch(row + stride);
+    fetch_y(row + stride);
     if (a.y) {
       if (a.norm_post) {
         const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(b), part[0]), p.inv_d, a.eps));
@@ -212,6 +215,7 @@ __global__ void __launch_bounds__(NormCfg<NCH>::T, NormCfg<NCH>::BLOCKS)
 #pragma unroll
       for (int k = 0; k < NCH; ++k) store8<FULL>(o, 8 * (k * T + t), d, p.vec & kVecHOut, h[k]);
     }
+    fetch_h(row + stride);  // here, where the branch's registers are free again
     if (!a.n_out && !a.out.codes) continue;
     if (a.norm_pre) {
       const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(h), part[1]), p.inv_d, a.eps));
