@@ -104,11 +104,13 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
                :
                : "memory");
 }
-// The same for two sets.
-__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[2][16]) {
+// The same for four sets.
+__device__ __forceinline__ void tmem_wait64(uint32_t (&r)[4][16]) {
   tmem_wait16(r[0]);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[1][i])::"memory");
+  for (int j = 1; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[j][i])::"memory");
 }
 
 // A tile of this CTA's shared memory to global memory (the map's box and swizzle);
@@ -180,14 +182,14 @@ struct ManyCfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = 4;
   static constexpr int EPI_STAGE = 2048;  // per epilogue warp: a 32-row x 64-byte block on its way to y
-  // One warpgroup for the producer, the MMA issuer and two idle warps, four
-  // for the epilogue: a block's waits, scales and arrivals cost each warp as
-  // many cycles as its sums, so four warps per scheduler take turns.  The
-  // registers of a launch at 96 a thread are shared out as 32 and 112:
-  // 128 * 32 + 512 * 112 <= 640 * 96.
-  static constexpr int EPI_WARPS = 16, THREADS = 128 + 32 * EPI_WARPS;
-  static constexpr int COLS = BN / (EPI_WARPS / 4);  // columns of one epilogue warp
-  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * EPI_STAGE + 1024;
+  // One warpgroup for the producer, the MMA issuer and the two scale warps,
+  // two for the epilogue.  The registers of a launch at 168 a thread are
+  // shared out as 56 and 216: 128 * 56 + 256 * 216 <= 384 * 168.  (Sixteen
+  // epilogue warps of 64 columns took as long.)
+  static constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
+  static constexpr int SCALE_SLOTS = 4;  // blocks whose scale products are in shared memory
+  static constexpr int SCALE_BYTES = SCALE_SLOTS * 2 * BM * 4;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * EPI_STAGE + SCALE_BYTES + 1024;
   static_assert(SMEM + 1024 <= 232448, "over 227 KB of shared memory");
   static constexpr int GROUP_M = 16;      // row blocks that share the output blocks in L2
 };
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
                          const __grid_constant__ Fp8GemmArgs a) {
   using C = ManyCfg;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[C::STAGES], bar_done[C::STAGES], bar_acce[2];
+  __shared__ __align__(8) uint64_t bar_full[C::STAGES], bar_done[C::STAGES], bar_acce[2], bar_scale[C::SCALE_SLOTS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -219,6 +221,7 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       mbar_init(&bar_done[s], 1);
     }
     for (int b = 0; b < 2; ++b) mbar_init(&bar_acce[b], C::EPI_WARPS);
+    for (int s = 0; s < C::SCALE_SLOTS; ++s) mbar_init(&bar_scale[s], 2);
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -228,9 +231,10 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  float* scales = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + C::EPI_WARPS * C::EPI_STAGE);
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && lane == 0) {
       uint32_t it = 0;
       bool ok = true;
@@ -259,7 +263,8 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
     }
     if (warp == 1) {
       // bar_done of a stage tells both that the stage is free and that the
-      // block's sums are complete.
+      // block's sums are complete; the epilogue waits for every one, so no
+      // arrival is on its way when the CTA exits.
       constexpr uint32_t idesc = idesc_e4m3_f32(C::BM, C::BN);
       const uint64_t dbase = desc_k_sw128(smem_u32(smem));
       const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
@@ -278,91 +283,112 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         full = mbar_test(&bar_full[(it + 1) % C::STAGES], ((it + 1) / C::STAGES) & 1);
         free = mbar_test(&bar_acce[b ^ 1], (((it + 1) >> 1) & 1) ^ 1);
       }
-      // The last arrivals land before the CTA can exit.
-      if (it == total)
-        for (uint32_t j = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; j < it; ++j)
-          if (!warp_wait(&bar_done[j % C::STAGES], (j / C::STAGES) & 1, a.err, kErrWaitDrain, &abort_flag)) break;
+    }
+    if (warp >= 2) {
+      // Scale products of one output block (half of the tile): slot it % 4
+      // takes sx[row] * sw for the 128 rows once the epilogue is done with
+      // block it - 2 (so with it - 4, the slot's last).  Loads run two blocks
+      // ahead.  In the epilogue's own threads these loads and their
+      // bookkeeping took 200 cycles of every block.
+      const int half = warp - 2;
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+        int mb, nb;
+        tile_of(tile, tiles_m, tiles_n, mb, nb);
+        const float* sw = a.sw + (long)min(2 * nb + half, oblocks - 1) * kblocks;
+        const float* sx[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sx[j] = a.sx + min((long)mb * C::BM + 32 * j + lane, a.rows - 1);
+        float x[2][4], w[2];
+        auto fetch = [&](int kb, int to) {
+          const int k = min(kb, kblocks - 1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[to][j] = __ldg(sx[j] + (long)k * a.lds);
+          w[to] = __ldg(sw + k);
+        };
+        auto put = [&](int kb, int from) {
+          if (!warp_wait(&bar_acce[it & 1], ((it >> 1) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag)) return false;
+          float* to = scales + (it % C::SCALE_SLOTS) * 2 * C::BM + half * C::BM + lane;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[32 * j] = x[from][j] * w[from];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_scale[it % C::SCALE_SLOTS]);
+          ++it;
+          fetch(kb + 2, from);
+          return true;
+        };
+        fetch(0, 0);
+        fetch(1, 1);
+        for (int kb = 0; kb < kblocks && ok; kb += 2) {
+          ok = put(kb, 0);
+          if (ok && kb + 1 < kblocks) ok = put(kb + 1, 1);
+        }
+      }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // Epilogue: warp w holds TMEM lanes 32 (w % 4) .. + 31, one row of x per
-    // thread, and a quarter of the tile's columns.
-    const int q = warp & 3, quarter = (warp - 4) >> 2;
+    // thread, and one half (one output block) of the tile's columns.
+    const int q = warp & 3, half = (warp - 4) >> 2;
     uint8_t* stage = smem + C::STAGES * C::STAGE_BYTES + (warp - 4) * C::EPI_STAGE;
-    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + quarter * C::COLS;
+    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + half * 128;
+    const float* scale = scales + half * C::BM + 32 * q + lane;
     uint32_t it = 0;
-    bool ok = true, done = false;  // done: the next block's barrier, tested ahead
+    bool ok = true, done = false, scaled = false;  // the next block's barriers, tested ahead
     for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
       int mb, nb;
       tile_of(tile, tiles_m, tiles_n, mb, nb);
       const long row0 = (long)mb * C::BM + 32 * q;
-      const float* sx = a.sx + min(row0 + lane, a.rows - 1);
-      const int col0 = nb * C::BN + quarter * C::COLS, ob = col0 / kFp8Block;
-      const float* sw = a.sw + (long)min(ob, oblocks - 1) * kblocks;
-      uint64_t acc[C::COLS / 2];  // column pairs
+      const int col0 = nb * C::BN + half * 128;
+      float acc[128];
 #pragma unroll
-      for (int i = 0; i < C::COLS / 2; ++i) acc[i] = 0;
+      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
       if (a.bias) {  // padded with zeros to whole tiles
-        const ulonglong2* bp = reinterpret_cast<const ulonglong2*>(a.bias + col0);
+        const float4* bp = reinterpret_cast<const float4*>(a.bias + col0);
 #pragma unroll
-        for (int i = 0; i < C::COLS / 4; ++i) {
-          const ulonglong2 b2 = __ldg(bp + i);
-          acc[2 * i] = b2.x;
-          acc[2 * i + 1] = b2.y;
+        for (int i = 0; i < 32; ++i) {
+          const float4 f = __ldg(bp + i);
+          acc[4 * i] = f.x, acc[4 * i + 1] = f.y, acc[4 * i + 2] = f.z, acc[4 * i + 3] = f.w;
         }
       }
-      // The scales of two blocks are in hand, those of the next two on their
-      // way (a load is about two blocks' time away).
-      float x0 = __ldg(sx), x1 = __ldg(sx + (long)min(1, kblocks - 1) * a.lds), x2, x3;
-      float w0 = __ldg(sw), w1 = __ldg(sw + min(1, kblocks - 1)), w2, w3;
-      auto fetch = [&](int kb) {
-        const int k2 = min(kb, kblocks - 1), k3 = min(kb + 1, kblocks - 1);
-        x2 = __ldg(sx + (long)k2 * a.lds);
-        x3 = __ldg(sx + (long)k3 * a.lds);
-        w2 = __ldg(sw + k2);
-        w3 = __ldg(sw + k3);
-      };
-      fetch(2);
       for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const float s = (kb & 1) ? x1 * w1 : x0 * w0;
-        if (kb & 1) {
-          x0 = x2, x1 = x3, w0 = w2, w1 = w3;
-          fetch(kb + 3);
-        }
-        const uint64_t ss = pack_f32x2(s, s);
         const uint32_t b = it & 1, src = tm + b * C::BN;
-        ok = warp_wait(done, &bar_done[it % C::STAGES], (it / C::STAGES) & 1, a.err, kErrWaitAccFull, &abort_flag);
+        ok = warp_wait(scaled, &bar_scale[it % C::SCALE_SLOTS], (it / C::SCALE_SLOTS) & 1, a.err, kErrWaitFull, &abort_flag) &&
+             warp_wait(done, &bar_done[it % C::STAGES], (it / C::STAGES) & 1, a.err, kErrWaitAccFull, &abort_flag);
         if (!ok) break;
+        const float s = scale[(it % C::SCALE_SLOTS) * 2 * C::BM];
         tc_fence_after();
-        // 16 columns at a time through two register blocks: the buffer goes
+        // 16 columns at a time through four register blocks: the buffer goes
         // back to the MMA issuer once the last block is loaded, with half of
-        // the sums still to be added.
-        uint32_t r[2][16];
+        // the sums still to be added.  (Single fma: pairs of f32 in one
+        // instruction took 14 % longer here.)
+        uint32_t r[4][16];
+        auto load = [&](int c) { tmem_ld16(src + 16 * c, r[c & 3]); };
         auto add = [&](int c) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) fma_f32x2(acc[8 * c + i], pack_u32x2(r[c & 1][2 * i], r[c & 1][2 * i + 1]), ss);
+          for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(__uint_as_float(r[c & 3][i]), s, acc[16 * c + i]);
         };
-        tmem_ld16(src, r[0]);
-        tmem_ld16(src + 16, r[1]);
-        tmem_wait32(r);
-        add(0);
-        tmem_ld16(src + 32, r[0]);
-        add(1);
-        tmem_ld16(src + 48, r[1]);
-        tmem_wait32(r);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) load(c);
+        tmem_wait64(r);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          add(c);
+          load(c + 4);
+        }
+        tmem_wait64(r);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_acce[b]);
         done = mbar_test(&bar_done[(it + 1) % C::STAGES], ((it + 1) / C::STAGES) & 1);
-        add(2);
-        add(3);
+        scaled = mbar_test(&bar_scale[(it + 1) % C::SCALE_SLOTS], ((it + 1) / C::SCALE_SLOTS) & 1);
+#pragma unroll
+        for (int c = 4; c < 8; ++c) add(c);
       }
       if (!ok) break;
       const int nrows = (int)min(32l, a.rows - row0);
       if (nrows <= 0 || col0 >= a.out) continue;
-      float v[C::COLS];
-#pragma unroll
-      for (int i = 0; i < C::COLS / 2; ++i) unpack_f32x2(acc[i], v[2 * i], v[2 * i + 1]);
       if (a.y_vec) {
         // 64 bytes of each of the warp's 32 rows at a time, through shared
         // memory (64-byte swizzle: 16-byte chunk c of row r at c ^ (r / 2 & 3))
@@ -379,18 +405,18 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         };
         if (a.y_dtype == G4M_F32) {
 #pragma unroll
-          for (int c = 0; c < C::COLS / 16; ++c) {
+          for (int c = 0; c < 128 / 16; ++c) {
             if (col0 + 16 * c >= a.out) break;
             uint4 o[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              o[i] = make_uint4(__float_as_uint(v[16 * c + 4 * i]), __float_as_uint(v[16 * c + 4 * i + 1]),
-                                __float_as_uint(v[16 * c + 4 * i + 2]), __float_as_uint(v[16 * c + 4 * i + 3]));
+              o[i] = make_uint4(__float_as_uint(acc[16 * c + 4 * i]), __float_as_uint(acc[16 * c + 4 * i + 1]),
+                                __float_as_uint(acc[16 * c + 4 * i + 2]), __float_as_uint(acc[16 * c + 4 * i + 3]));
             send(o, col0 + 16 * c);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < C::COLS / 32; ++c) {
+          for (int c = 0; c < 128 / 32; ++c) {
             if (col0 + 32 * c >= a.out) break;
             uint4 o[4];
 #pragma unroll
@@ -398,7 +424,7 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
               uint32_t w[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float f0 = v[32 * c + 8 * i + 2 * j], f1 = v[32 * c + 8 * i + 2 * j + 1];
+                const float f0 = acc[32 * c + 8 * i + 2 * j], f1 = acc[32 * c + 8 * i + 2 * j + 1];
                 w[j] = a.y_dtype == G4M_BF16 ? pack2(f0, f1, __nv_bfloat16()) : pack2(f0, f1, __half());
               }
               o[i] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -410,8 +436,8 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         with_type(a.y_dtype, [&](auto* tp) {
           auto* y = static_cast<decltype(tp)>(a.y) + (row0 + lane) * a.ldy + col0;
 #pragma unroll
-          for (int i = 0; i < C::COLS; ++i)
-            if (col0 + i < a.out) from_f32(v[i], y + i);
+          for (int i = 0; i < 128; ++i)
+            if (col0 + i < a.out) from_f32(acc[i], y + i);
         });
       }
     }
@@ -432,8 +458,10 @@ template <int NT>
 struct FewCfg {
   static constexpr int W_BYTES = kFp8TileBytes, X_BYTES = NT * 128;
   static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
-  static constexpr int STAGES = NT == 16 ? 5 : NT == 64 ? 3 : 4;
-  static constexpr int BUFS = NT == 16 ? 8 : NT == 32 ? 8 : NT == 64 ? 4 : 2;  // accumulators in flight
+  // Two CTAs fit an SM.  (Twice the stages for grids of one CTA per SM gained
+  // nothing, and cost half a microsecond a launch.)
+  static constexpr int STAGES = NT == 16 ? 5 : NT == 32 ? 4 : 3;
+  static constexpr int BUFS = NT == 64 ? 4 : 8;  // accumulators in flight
   static constexpr int TMEM_COLS = BUFS * NT;
   // An epilogue warp holds 32 outputs of up to 32 rows: one warpgroup for each
   // 32 rows (with 64 rows in a warp, a block's sums took 925 cycles).
@@ -443,14 +471,13 @@ struct FewCfg {
   static constexpr int PART_BYTES = NT * 128 * 4;  // partial totals from the cluster: splits * ceil(rows / splits) <= NT rows, splits a power of 2
   static constexpr int BARS = 2 * STAGES + 2 * BUFS + 1;
   static constexpr int THREADS = 64 + 128 * GROUPS;
-  static constexpr int CTAS = NT <= 64 ? 2 : 1;  // per SM
   static constexpr int SMEM = STAGES * STAGE_BYTES + SCALE_BYTES + PART_BYTES + 1024;
   static_assert(NT * 512 <= STAGES * STAGE_BYTES, "the outgoing totals reuse the stages");
-  static_assert(CTAS * TMEM_COLS <= 512 && CTAS * (SMEM + 1024 + 512) <= 233472, "over the SM's memories");
+  static_assert(2 * TMEM_COLS <= 512 && 2 * (SMEM + 1024 + 512) <= 233472, "over the SM's memories");
 };
 
 template <int NT>
-__global__ void __launch_bounds__(FewCfg<NT>::THREADS, FewCfg<NT>::CTAS)
+__global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
     fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ Fp8GemmArgs a, int splits) {
   using C = FewCfg<NT>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -492,8 +519,8 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, FewCfg<NT>::CTAS)
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
       const uint8_t* w = a.w + ((long)ob * kblocks + k0) * kFp8TileBytes;
+      int it = 0;
       for (; it < nk; ++it) {
         const int s = it % C::STAGES;
         // An earlier kernel on this device failed: looked up once the first
@@ -505,14 +532,12 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, FewCfg<NT>::CTAS)
         bulk_load(sw, w + (long)it * kFp8TileBytes, C::W_BYTES, &bar_full[s]);
         tma_load_2d(sw + C::W_BYTES, &mx, &bar_full[s], (k0 + it) * kFp8Block, (int)row0);
       }
-      for (int j = it > C::STAGES ? it - C::STAGES : 0; j < it; ++j)
-        drain(&bar_full[j % C::STAGES], (j / C::STAGES) & 1, a.err);
+      for (int j = max(it - C::STAGES, 0); j < it; ++j) drain(&bar_full[j % C::STAGES], (j / C::STAGES) & 1, a.err);
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc = idesc_e4m3_f32(128, NT);
     const uint64_t dbase = desc_k_sw128(smem_u32(smem));
-    int it = 0;
-    for (; it < nk; ++it) {
+    for (int it = 0; it < nk; ++it) {
       const int s = it % C::STAGES, b = it % C::BUFS;
       const uint64_t dw = desc_add(dbase, s * C::STAGE_BYTES);
       if (!warp_wait(&bar_acce[b], ((it / C::BUFS) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag) ||
@@ -520,11 +545,10 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, FewCfg<NT>::CTAS)
         break;
       tc_fence_after();
       mma_block(tmem_base + b * NT, dw, desc_add(dw, C::W_BYTES), idesc, &bar_accf[b]);
-      mma_commit_elected(&bar_empty[s]);
+      // Only for a stage that is filled again: every arrival is waited for, so
+      // none is on its way when the CTA exits.
+      if (it + C::STAGES < nk) mma_commit_elected(&bar_empty[s]);
     }
-    if (it == nk)  // the last stage-release arrivals land before the CTA can exit
-      for (int j = it > C::STAGES ? it - C::STAGES : 0; j < it; ++j)
-        if (!warp_wait(&bar_empty[j % C::STAGES], (j / C::STAGES) & 1, a.err, kErrWaitDrain, &abort_flag)) break;
   } else {
     const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + r0;
     const float* swp = a.sw + (long)ob * kblocks + k0;
@@ -681,7 +705,8 @@ cudaError_t fp8_weight_tiles(const uint8_t* w, int out, int in, uint8_t* tiles, 
 // ---------------------------------------------------------------------------
 template <int NT>
 static cudaError_t setup_few() {
-  return cudaFuncSetAttribute(fp8_gemm_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<NT>::SMEM);
+  using C = FewCfg<NT>;
+  return cudaFuncSetAttribute(fp8_gemm_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
 }
 
 cudaError_t fp8_gemm_setup() {
@@ -689,7 +714,6 @@ cudaError_t fp8_gemm_setup() {
   if (e == cudaSuccess) e = setup_few<16>();
   if (e == cudaSuccess) e = setup_few<32>();
   if (e == cudaSuccess) e = setup_few<64>();
-  if (e == cudaSuccess) e = setup_few<128>();
   return e;
 }
 
@@ -698,12 +722,19 @@ static cudaError_t launch_few(const Fp8GemmArgs& a, int sms, cudaStream_t st) {
   using C = FewCfg<NT>;
   CUtensorMap mx;
   if (!make_tmap_u8_pitch(&mx, a.x, a.rows, a.in, a.ldx, NT)) return cudaErrorInvalidValue;
-  const long units = fp8_blocks(a.out) * ((a.rows + NT - 1) / NT), kblocks = fp8_blocks(a.in);
-  // Split the column blocks until the CTAs fill the SMs.
+  const long row_tiles = (a.rows + NT - 1) / NT, units = fp8_blocks(a.out) * row_tiles, kblocks = fp8_blocks(a.in);
+  // Split the column blocks while the CTAs stay about as many as the SMs and
+  // keep four blocks each, or fewer where they would leave most SMs idle.
+  // (1 x 4096 -> 4096: 11.7 us unsplit, 8.6 / 7.1 / 8.2 split by 2 / 4 / 8;
+  // 1 x 1536 -> 12288, 96 CTAs unsplit: 7.5, and 8.6 split by 2; 100 x 768 ->
+  // 2304: 5.9, and 7.8 split by 2; 1 x 768 -> 768: 5.1, and 4.3 split by 4.)
   int splits = 1;
-  while (splits < 8 && 2 * splits <= kblocks && units * splits < sms) splits *= 2;
+  while (splits < 8 && 2 * splits * units <= sms + sms / 8 && 2 * splits <= kblocks &&
+         (8 * splits <= kblocks || 8 * splits * units <= sms))
+    splits *= 2;
+  if (units * splits > 0x7fffffffL || row_tiles > 65535) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(fp8_blocks(a.out) * splits), (unsigned)((a.rows + NT - 1) / NT));
+  cfg.gridDim = dim3((unsigned)(fp8_blocks(a.out) * splits), (unsigned)row_tiles);
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = st;
@@ -712,16 +743,18 @@ static cudaError_t launch_few(const Fp8GemmArgs& a, int sms, cudaStream_t st) {
   at[0].val.clusterDim.x = splits;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, fp8_gemm_few_kernel<NT>, mx, a, splits);
 }
 
 cudaError_t fp8_gemm(const Fp8GemmArgs& a, int dev, cudaStream_t st) {
   const int sms = g_num_sms(dev);
+  // Few rows while one CTA per SM covers all tiles, in the smallest tile that
+  // does; beyond that the 128 x 256 tiles read less for each product.
+  auto fits = [&](int nt) { return fp8_blocks(a.out) * ((a.rows + nt - 1) / nt) <= sms; };
   if (a.rows <= 16) return launch_few<16>(a, sms, st);
-  if (a.rows <= 32) return launch_few<32>(a, sms, st);
-  if (a.rows <= 64) return launch_few<64>(a, sms, st);
-  if (a.rows <= 256) return launch_few<128>(a, sms, st);
+  if (a.rows <= 32 || fits(32)) return launch_few<32>(a, sms, st);
+  if (a.rows <= 64 || fits(64)) return launch_few<64>(a, sms, st);
   CUtensorMap mx, my;
   if (!make_tmap_u8_pitch(&mx, a.x, a.rows, a.in, a.ldx, ManyCfg::BM)) return cudaErrorInvalidValue;
   if (!a.y_vec) my = mx;  // not used
