@@ -52,14 +52,6 @@ __device__ __forceinline__ void mma_block(uint32_t d_tmem, uint64_t adesc, uint6
       : "memory");
 }
 
-// Whole warp: the elected lane's arrival on `bar` once its MMAs so far are done.
-__device__ __forceinline__ void mma_commit_elected(uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
-      : "memory");
-}
-
 // Whether the phase is complete, without waiting (try_wait may suspend the thread).
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -485,24 +477,38 @@ struct FewCfg {
   // Two CTAs fit an SM.  (Twice the stages for grids of one CTA per SM gained
   // nothing, and cost half a microsecond a launch.)
   static constexpr int STAGES = NT == 16 ? 5 : NT == 32 ? 4 : 3;
-  static constexpr int BUFS = NT == 64 ? 4 : 8;  // accumulators in flight
-  static constexpr int TMEM_COLS = BUFS * NT;
+  // One accumulator per stage: bar_done of a stage stands for both, and no
+  // wait on it can fall a whole turn behind.
+  static constexpr int TMEM_COLS = STAGES * NT <= 128 ? 128 : 256;
   // An epilogue warp holds 32 outputs of up to 32 rows: one warpgroup for each
   // 32 rows (with 64 rows in a warp, a block's sums took 925 cycles).
   static constexpr int RP = NT < 32 ? NT : 32, GROUPS = NT / RP;
   static constexpr int SCALE_BLOCKS = NT == 16 ? 8 : NT == 32 ? 4 : 2;  // column blocks whose row scales are fetched together
   static constexpr int SCALE_BYTES = 4 * 2 * SCALE_BLOCKS * NT * 4;     // per epilogue warp, double-buffered
   static constexpr int PART_BYTES = NT * 128 * 4;  // partial totals from the cluster: splits * ceil(rows / splits) <= NT rows, splits a power of 2
-  static constexpr int BARS = 2 * STAGES + 2 * BUFS + 1;
+  static constexpr int BARS = 3 * STAGES + 1;
   static constexpr int THREADS = 64 + 128 * GROUPS;
   static constexpr int SMEM = STAGES * STAGE_BYTES + SCALE_BYTES + PART_BYTES + 1024;
   static_assert(NT * 512 <= STAGES * STAGE_BYTES, "the outgoing totals reuse the stages");
   static_assert(2 * TMEM_COLS <= 512 && 2 * (SMEM + 1024 + 512) <= 233472, "over the SM's memories");
 };
 
+// Rows first, first + step, ... of n: the S partial totals, [rank][row][128],
+// added in rank order.
+template <int S, int STEP, class T>
+__device__ __forceinline__ void add_parts(const float* part, int n, int first, float bias, T* y, long ldy) {
+#pragma unroll 4
+  for (int j = first; j < n; j += STEP) {
+    float total = part[j * 128];
+#pragma unroll
+    for (int p = 1; p < S; ++p) total += part[(p * n + j) * 128];
+    from_f32(total + bias, y + j * ldy);
+  }
+}
+
 template <int NT>
 __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
-    fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ Fp8GemmArgs a, int splits) {
+    fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ Fp8GemmArgs a, int lg) {
   using C = FewCfg<NT>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[C::BARS];
@@ -511,17 +517,20 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kblocks = (a.in + kFp8Block - 1) / kFp8Block;
-  const int rank = splits > 1 ? (int)cluster_rank() : 0;
-  const int ob = blockIdx.x / splits;
+  // The cluster's CTAs split the column blocks: 2^lg of them, so that nothing
+  // here is a division.
+  const int splits = 1 << lg, rank = lg ? (int)cluster_rank() : 0;
+  const int ob = blockIdx.x >> lg;
   const long row0 = (long)blockIdx.y * NT;
   const int nrows = (int)min((long)NT, a.rows - row0);
-  const int k0 = (int)((long)kblocks * rank / splits), nk = (int)((long)kblocks * (rank + 1) / splits) - k0;
+  const int k0 = (int)((long)kblocks * rank >> lg), nk = (int)((long)kblocks * (rank + 1) >> lg) - k0;
   // The rows that this CTA of the cluster completes.
-  const int j0 = nrows * rank / splits, j1 = nrows * (rank + 1) / splits;
+  const int j0 = nrows * rank >> lg, j1 = nrows * (rank + 1) >> lg;
   float* part = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES);
 
-  uint64_t *bar_full = bars, *bar_empty = bars + C::STAGES, *bar_accf = bars + 2 * C::STAGES, *bar_acce = bar_accf + C::BUFS,
-           *bar_part = bars + C::BARS - 1;
+  // bar_done of a stage tells both that the stage is free and that the block's
+  // sums are complete.
+  uint64_t *bar_full = bars, *bar_done = bars + C::STAGES, *bar_acce = bars + 2 * C::STAGES, *bar_part = bars + C::BARS - 1;
   if (threadIdx.x < C::BARS) {
     mbar_init(bars + threadIdx.x, bars + threadIdx.x >= bar_acce && bars + threadIdx.x < bar_part ? 4 * C::GROUPS : 1);
     fence_mbar_init();
@@ -550,7 +559,7 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
         // An earlier kernel on this device failed: looked up once the first
         // copies are on their way.
         if (it == C::STAGES && *reinterpret_cast<volatile int*>(a.err) != 0) abort_flag = 1;
-        if (!mbar_wait(&bar_empty[s], ((it / C::STAGES) & 1) ^ 1, a.err, kErrWaitEmpty, &abort_flag)) break;
+        if (!mbar_wait(&bar_done[s], ((it / C::STAGES) & 1) ^ 1, a.err, kErrWaitEmpty, &abort_flag)) break;
         uint8_t* sw = smem + s * C::STAGE_BYTES;
         mbar_expect_tx(&bar_full[s], C::STAGE_BYTES);
         bulk_load(sw, w + (long)it * kFp8TileBytes, C::W_BYTES, &bar_full[s]);
@@ -562,16 +571,14 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
     constexpr uint32_t idesc = idesc_e4m3_f32(128, NT);
     const uint64_t dbase = desc_k_sw128(smem_u32(smem));
     for (int it = 0; it < nk; ++it) {
-      const int s = it % C::STAGES, b = it % C::BUFS;
+      const int s = it % C::STAGES;
+      const uint32_t turn = (it / C::STAGES) & 1;
       const uint64_t dw = desc_add(dbase, s * C::STAGE_BYTES);
-      if (!warp_wait(&bar_acce[b], ((it / C::BUFS) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag) ||
-          !warp_wait(&bar_full[s], (it / C::STAGES) & 1, a.err, kErrWaitFull, &abort_flag))
+      if (!warp_wait(&bar_acce[s], turn ^ 1, a.err, kErrWaitAccEmpty, &abort_flag) ||
+          !warp_wait(&bar_full[s], turn, a.err, kErrWaitFull, &abort_flag))
         break;
       tc_fence_after();
-      mma_block(tmem_base + b * NT, dw, desc_add(dw, C::W_BYTES), idesc, &bar_accf[b]);
-      // Only for a stage that is filled again: every arrival is waited for, so
-      // none is on its way when the CTA exits.
-      if (it + C::STAGES < nk) mma_commit_elected(&bar_empty[s]);
+      mma_block(tmem_base + s * NT, dw, desc_add(dw, C::W_BYTES), idesc, &bar_done[s]);
     }
   } else {
     const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + r0;
@@ -606,8 +613,8 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
       const float w = __shfl_sync(0xffffffffu, wl, i & 31);
       const uint64_t ww = pack_f32x2(w, w);
       const float* s = sc + (i / SB & 1) * SB * C::RP + i % SB * C::RP;
-      const int b = i % C::BUFS;
-      if (!warp_wait(&bar_accf[b], (i / C::BUFS) & 1, a.err, kErrWaitAccFull, &abort_flag)) break;
+      const int b = i % C::STAGES;
+      if (!warp_wait(&bar_done[b], (i / C::STAGES) & 1, a.err, kErrWaitAccFull, &abort_flag)) break;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < C::RP / 16; ++c) {
@@ -663,7 +670,7 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
     cluster_wait();
     if (warp >= 2) {
       if (warp == 2 && lane < splits) {
-        const int begin = nrows * lane / splits, n = nrows * (lane + 1) / splits - begin;
+        const int begin = nrows * lane >> lg, n = (nrows * (lane + 1) >> lg) - begin;
         if (n > 0)
           cluster_push(cluster_map(smem_u32(part + rank * n * 128), lane), smem + begin * 512, n * 512,
                        cluster_map(smem_u32(bar_part), lane));
@@ -672,19 +679,10 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
       ok = warp_wait(bar_part, 0, a.err, kErrWaitAccFull, &abort_flag);
       if (ok && o < a.out)
         with_type(a.y_dtype, [&](auto* tp) {
-          auto* y = static_cast<decltype(tp)>(a.y) + row0 * a.ldy + o;
-#pragma unroll 2
-          for (int j = j0 + group; j < j1; j += C::GROUPS) {
-            const float* from = part + (j - j0) * 128 + t;
-            float v[8];
-#pragma unroll
-            for (int p = 0; p < 8; ++p) v[p] = p < splits ? from[p * (j1 - j0) * 128] : 0.0f;
-            float total = v[0];
-#pragma unroll
-            for (int p = 1; p < 8; ++p)
-              if (p < splits) total += v[p];
-            from_f32(total + bias, y + j * a.ldy);
-          }
+          auto* y = static_cast<decltype(tp)>(a.y) + (row0 + j0) * a.ldy + o;
+          if (lg == 1) add_parts<2, C::GROUPS>(part + t, j1 - j0, group, bias, y, a.ldy);
+          else if (lg == 2) add_parts<4, C::GROUPS>(part + t, j1 - j0, group, bias, y, a.ldy);
+          else add_parts<8, C::GROUPS>(part + t, j1 - j0, group, bias, y, a.ldy);
         });
     }
     // No CTA leaves while another one may still push to it.
@@ -752,10 +750,11 @@ static cudaError_t launch_few(const Fp8GemmArgs& a, int sms, cudaStream_t st) {
   // (1 x 4096 -> 4096: 11.7 us unsplit, 8.6 / 7.1 / 8.2 split by 2 / 4 / 8;
   // 1 x 1536 -> 12288, 96 CTAs unsplit: 7.5, and 8.6 split by 2; 100 x 768 ->
   // 2304: 5.9, and 7.8 split by 2; 1 x 768 -> 768: 5.1, and 4.3 split by 4.)
-  int splits = 1;
-  while (splits < 8 && 2 * splits * units <= sms + sms / 8 && 2 * splits <= kblocks &&
-         (8 * splits <= kblocks || 8 * splits * units <= sms))
-    splits *= 2;
+  int lg = 0;
+  while (lg < 3 && (units << (lg + 1)) <= sms + sms / 8 && (2 << lg) <= kblocks &&
+         ((8 << lg) <= kblocks || (units << (lg + 3)) <= sms))
+    ++lg;
+  const int splits = 1 << lg;
   if (units * splits > 0x7fffffffL || row_tiles > 65535) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(fp8_blocks(a.out) * splits), (unsigned)row_tiles);
@@ -768,7 +767,7 @@ static cudaError_t launch_few(const Fp8GemmArgs& a, int sms, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = splits > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, fp8_gemm_few_kernel<NT>, mx, a, splits);
+  return cudaLaunchKernelEx(&cfg, fp8_gemm_few_kernel<NT>, mx, a, lg);
 }
 
 cudaError_t fp8_gemm(const Fp8GemmArgs& a, int dev, cudaStream_t st) {
