@@ -11,7 +11,7 @@
 // neighbouring heads, so that it reads and writes contiguous memory.  For
 // 16384 tokens x 40 heads x 128 bf16 (335 MB): 73 us with one head per thread
 // and step but four tokens per warp, 71 us with the angles read from shared
-// memory for every head, 58 us as it is.
+// memory for every head, 60 us as it is.
 #include <algorithm>
 
 #include "fp8_rows.cuh"
@@ -65,9 +65,21 @@ struct RopeChunk {
   }
 };
 
-// VEC: every head starts on a 16-byte boundary and the pairs come in whole
-// chunks of 8; a thread then turns 8 pairs of a head.  Otherwise it turns one.
-template <class T, bool VEC, bool INTERLEAVED>
+// Cosines and sines of the block's tokens.
+__device__ __forceinline__ void rope_table(const RopeArgs& a, float2* cs, long t0, int nt) {
+  for (int i = threadIdx.x; i < nt * a.half; i += blockDim.x) {
+    const int t = i / a.half, j = i - t * a.half;
+    const long pos = a.pos64 ? static_cast<const long*>(a.positions)[t0 + t] : static_cast<const int*>(a.positions)[t0 + t];
+    const uint64_t phase = (uint64_t)pos * a.turns[j];
+    float sn, cn;
+    sincospif(__ll2float_rn((long long)phase) * 0x1p-63f, &sn, &cn);  // half turns in [-1, 1]
+    cs[i] = make_float2(cn * a.scale, sn * a.scale);
+  }
+}
+
+// Every head starts on a 16-byte boundary and the pairs come in whole chunks
+// of 8: a thread turns 8 pairs of a head.
+template <class T, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeLaunch l) {
   extern __shared__ float4 cs4[];
   float2* cs = reinterpret_cast<float2*>(cs4);
@@ -75,7 +87,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
   const long t0 = (long)blockIdx.x * l.token_block;
   const int nt = (int)min((long)l.token_block, a.tokens - t0);
   const int heads = a.v[0].heads + a.v[1].heads;
-  const int turn_items = VEC ? a.half / 8 : a.half;
+  const int turn_items = a.half / 8;
   // Work of a thread: (token, lane, item), heads h0, h0 + step, ...
   const int step = l.lanes * gridDim.y, total = nt * l.lanes * l.items;
   int w = threadIdx.x, t, c, h0;
@@ -93,64 +105,41 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
     o = static_cast<T*>(v.out) + (t0 + t) * v.out_token_stride + head * v.out_head_stride;
     return k;
   };
-  // What a thread has in flight: one head's chunk, or four heads' elements.
-  constexpr int B = VEC ? 1 : 4;
   RopeChunk<T, INTERLEAVED> ka, kb;
-  T e0[B], e1[B];
   const T* x;
   T* o;
-  auto load_chunk = [&](int h, RopeChunk<T, INTERLEAVED>& k) {
+  auto load = [&](int h, RopeChunk<T, INTERLEAVED>& k) {
     if (h < heads) {
       head_of(h, x, o);
       k.load(x, 8 * c, a.half);
     }
   };
-  auto load_elements = [&](int h) {
-    const bool turns = c < turn_items;
-    const int iu = !turns ? a.half + c : INTERLEAVED ? 2 * c : c, iv = !turns ? iu : INTERLEAVED ? 2 * c + 1 : a.half + c;
-#pragma unroll
-    for (int i = 0; i < B; ++i)
-      if (h + i * step < heads) {
-        head_of(h + i * step, x, o);
-        e0[i] = x[iu];
-        e1[i] = x[iv];
-      }
-  };
   // The first loads go out before the angles are computed.
   if (w < total) {
     work_of();
-    if (VEC && c < turn_items) load_chunk(h0, ka);
-    if (!VEC) load_elements(h0);
+    if (c < turn_items) load(h0, ka);
   }
-  for (int i = threadIdx.x; i < nt * a.half; i += kRopeThreads) {
-    const int ti = i / a.half, j = i - ti * a.half;
-    const long pos = a.pos64 ? static_cast<const long*>(a.positions)[t0 + ti] : static_cast<const int*>(a.positions)[t0 + ti];
-    const uint64_t phase = (uint64_t)pos * a.turns[j];
-    float sn, cn;
-    sincospif(__ll2float_rn((long long)phase) * 0x1p-63f, &sn, &cn);  // half turns in [-1, 1]
-    cs[i] = make_float2(cn * a.scale, sn * a.scale);
-  }
+  rope_table(a, cs, t0, nt);
   __syncthreads();
   for (bool first = true; w < total; w += kRopeThreads, first = false) {
     if (!first) {
       work_of();
-      if (VEC && c < turn_items) load_chunk(h0, ka);
-      if (!VEC) load_elements(h0);
+      if (c < turn_items) load(h0, ka);
     }
-    if (VEC && c < turn_items) {
+    if (c < turn_items) {
       float2 r[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = cs[t * a.half + 8 * c + i];
       for (int h = h0; h < heads; h += 2 * step) {
-        load_chunk(h + step, kb);
+        load(h + step, kb);
         head_of(h, x, o);
         ka.turn(o, 8 * c, a.half, r);
         if (h + step >= heads) break;
-        load_chunk(h + 2 * step, ka);
+        load(h + 2 * step, ka);
         head_of(h + step, x, o);
         kb.turn(o, 8 * c, a.half, r);
       }
-    } else if (VEC) {  // columns that pass through
+    } else {  // columns that pass through
       const int e = 2 * a.half + 8 * (c - turn_items);
       for (int h = h0; h < heads; h += step) {
         if (!a.copy[head_of(h, x, o)]) continue;
@@ -163,49 +152,124 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
           for (int i = e; i < a.head_dim; ++i) o[i] = x[i];
         }
       }
-    } else {
-      const bool turns = c < turn_items;
-      const float2 r = turns ? cs[t * a.half + c] : make_float2(0.0f, 0.0f);
-      const int iu = !turns ? a.half + c : INTERLEAVED ? 2 * c : c, iv = INTERLEAVED ? 2 * c + 1 : a.half + c;
-      for (int h = h0;;) {
-#pragma unroll
-        for (int i = 0; i < B; ++i)
-          if (h + i * step < heads) {
-            const int k = head_of(h + i * step, x, o);
-            if (turns) {
-              const float u = to_f32(e0[i]), v = to_f32(e1[i]);
-              from_f32(u * r.x - v * r.y, o + iu);
-              from_f32(v * r.x + u * r.y, o + iv);
-            } else if (a.copy[k]) {
-              o[iu] = e0[i];
-            }
-          }
-        h += B * step;
-        if (h >= heads) break;
-        load_elements(h);
-      }
     }
   }
 }
 
-template <class T>
-static void launch_rope(const RopeLaunch& l, dim3 grid, cudaStream_t st) {
-  const size_t table = sizeof(float2) * l.token_block * l.a.half;
-  if (l.a.vec) {
-    if (l.a.interleaved) rope_kernel<T, true, true><<<grid, kRopeThreads, table, st>>>(l);
-    else rope_kernel<T, true, false><<<grid, kRopeThreads, table, st>>>(l);
+// Any other head: a warp brings a few whole heads into shared memory in the
+// widest words that all of them allow, turns their pairs there, and writes
+// them back in such words, the next heads on their way.  (Pair by pair from
+// global memory 3143 tokens x 24 heads x 172 f16, of which 34 turn, took 43 us
+// where this takes 11; 15568 x 24 x 110 bf16 70 and 53.)
+struct RopeStaged {
+  RopeArgs a;
+  int token_block, word, per;  // bytes of a word; heads of a batch
+  int flat;                    // the heads of a batch lie side by side: one run of words
+  int bytes[2], pitch, stage;  // of a head that move (all, or in place what turns); of a head, a batch in shared memory
+  int batches[2];              // of a token, per view
+  FastDiv by_half, by_batches, by_words[2];
+};
+
+template <int W>
+__device__ __forceinline__ void copy_word_async(void* dst, const void* src) {
+  if (W >= 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                 "n"(W >= 4 ? W : 4)
+                 : "memory");
   } else {
-    if (l.a.interleaved) rope_kernel<T, false, true><<<grid, kRopeThreads, table, st>>>(l);
-    else rope_kernel<T, false, false><<<grid, kRopeThreads, table, st>>>(l);
+    *static_cast<uint16_t*>(dst) = *static_cast<const uint16_t*>(src);
+  }
+}
+template <int W>
+__device__ __forceinline__ void copy_word(void* dst, const void* src) {
+  if (W == 16) *static_cast<uint4*>(dst) = *static_cast<const uint4*>(src);
+  else if (W == 8) *static_cast<uint2*>(dst) = *static_cast<const uint2*>(src);
+  else if (W == 4) *static_cast<uint32_t*>(dst) = *static_cast<const uint32_t*>(src);
+  else *static_cast<uint16_t*>(dst) = *static_cast<const uint16_t*>(src);
+}
+
+template <class T, bool INTERLEAVED, int W>
+__global__ void __launch_bounds__(kRopeThreads) rope_staged_kernel(const __grid_constant__ RopeStaged l) {
+  extern __shared__ float4 cs4[];
+  const RopeArgs& a = l.a;
+  float2* cs = reinterpret_cast<float2*>(cs4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int table = (l.token_block * a.half + 1) / 2 * 16;  // bytes, in whole 16
+  char* stage = reinterpret_cast<char*>(cs4) + table + warp * 2 * l.stage;
+  const long t0 = (long)blockIdx.x * l.token_block;
+  const int nt = (int)min((long)l.token_block, a.tokens - t0);
+  const int batches = l.batches[0] + l.batches[1], units = nt * batches, step = warps * gridDim.y;
+  struct Unit {
+    int t, k, h0, n;
+  };
+  auto unit_of = [&](int u) {
+    Unit r;
+    r.t = (int)div_by((uint32_t)u, l.by_batches);
+    const int b = u - r.t * batches;
+    r.k = b >= l.batches[0];
+    r.h0 = (b - (r.k ? l.batches[0] : 0)) * l.per;
+    r.n = min(l.per, a.v[r.k].heads - r.h0);
+    return r;
+  };
+  auto bring = [&](int u, char* to) {
+    if (u < units) {
+      const Unit r = unit_of(u);
+      const g4m_rope_view& v = a.v[r.k];
+      const char* x = reinterpret_cast<const char*>(static_cast<const T*>(v.x) + (t0 + r.t) * v.token_stride + r.h0 * v.head_stride);
+      if (l.flat) {
+        for (int i = lane * W; i < r.n * l.pitch; i += 32 * W) copy_word_async<W>(to + i, x + i);
+      } else {
+        const int words = l.bytes[r.k] / W;
+        for (int i = lane; i < r.n * words; i += 32) {
+          const int b = (int)div_by((uint32_t)i, l.by_words[r.k]), w = i - b * words;
+          copy_word_async<W>(to + b * l.pitch + w * W, x + b * v.head_stride * (long)sizeof(T) + w * W);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int u = blockIdx.y * warps + warp;
+  bring(u, stage);
+  rope_table(a, cs, t0, nt);
+  __syncthreads();
+  for (int buf = 0; u < units; u += step, buf ^= 1) {
+    char* s = stage + buf * l.stage;
+    bring(u + step, stage + (buf ^ 1) * l.stage);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const Unit r = unit_of(u);
+    for (int i = lane; i < r.n * a.half; i += 32) {
+      const int b = (int)div_by((uint32_t)i, l.by_half), j = i - b * a.half;
+      T* p = reinterpret_cast<T*>(s + b * l.pitch);
+      T &pu = p[INTERLEAVED ? 2 * j : j], &pv = p[INTERLEAVED ? 2 * j + 1 : a.half + j];
+      const float2 f = cs[r.t * a.half + j];
+      const float x = to_f32(pu), y = to_f32(pv);
+      from_f32(x * f.x - y * f.y, &pu);
+      from_f32(y * f.x + x * f.y, &pv);
+    }
+    __syncwarp();
+    const g4m_rope_view& v = a.v[r.k];
+    char* o = reinterpret_cast<char*>(static_cast<T*>(v.out) + (t0 + r.t) * v.out_token_stride + r.h0 * v.out_head_stride);
+    if (l.flat) {
+      for (int i = lane * W; i < r.n * l.pitch; i += 32 * W) copy_word<W>(o + i, s + i);
+    } else {
+      const int words = l.bytes[r.k] / W;
+      for (int i = lane; i < r.n * words; i += 32) {
+        const int b = (int)div_by((uint32_t)i, l.by_words[r.k]), w = i - b * words;
+        copy_word<W>(o + b * v.out_head_stride * (long)sizeof(T) + w * W, s + b * l.pitch + w * W);
+      }
+    }
+    __syncwarp();  // the buffer is free for the next but one
   }
 }
 
-cudaError_t rope_run(const RopeArgs& a, int dev, cudaStream_t st) {
+template <class T>
+static void launch_chunks(const RopeArgs& a, int sms, cudaStream_t st) {
   RopeLaunch l;
   l.a = a;
-  const int heads = a.v[0].heads + a.v[1].heads, sms = g_num_sms(dev);
+  const int heads = a.v[0].heads + a.v[1].heads;
   const int pass = a.copy[0] | a.copy[1] ? a.head_dim - 2 * a.half : 0;
-  l.items = a.vec ? a.half / 8 + (pass + 7) / 8 : a.half + pass;
+  l.items = a.half / 8 + (pass + 7) / 8;
   // Lanes enough that a warp covers one token's neighbouring heads, then as
   // many tokens as fill the block; short inputs take fewer tokens per block
   // and spread their heads over more lanes, then over more blocks.
@@ -219,9 +283,74 @@ cudaError_t rope_run(const RopeArgs& a, int dev, cudaStream_t st) {
   l.lanes = (int)(few ? std::max<long>(1, std::min<long>(heads, kRopeThreads / (tb * l.items))) : lanes);
   const long slices = std::max<long>(1, std::min<long>((heads + l.lanes - 1) / l.lanes, want / groups));
   const dim3 grid((unsigned)groups, (unsigned)slices);
-  if (a.dtype == G4M_F32) launch_rope<float>(l, grid, st);
-  else if (a.dtype == G4M_BF16) launch_rope<__nv_bfloat16>(l, grid, st);
-  else launch_rope<__half>(l, grid, st);
+  const size_t table = sizeof(float2) * l.token_block * a.half;
+  if (a.interleaved) rope_kernel<T, true><<<grid, kRopeThreads, table, st>>>(l);
+  else rope_kernel<T, false><<<grid, kRopeThreads, table, st>>>(l);
+}
+
+template <class T, int W>
+static void launch_staged_w(const RopeStaged& l, dim3 grid, int threads, size_t smem, cudaStream_t st) {
+  if (l.a.interleaved) rope_staged_kernel<T, true, W><<<grid, threads, smem, st>>>(l);
+  else rope_staged_kernel<T, false, W><<<grid, threads, smem, st>>>(l);
+}
+
+template <class T>
+static void launch_staged(const RopeArgs& a, int sms, cudaStream_t st) {
+  RopeStaged l;
+  l.a = a;
+  const int size = sizeof(T);
+  l.pitch = (a.head_dim * size + 15) / 16 * 16;
+  l.per = std::max(1, std::min(4, 2048 / l.pitch));
+  l.flat = 1;
+  for (int k = 0; k < 2; ++k) {
+    const g4m_rope_view& v = a.v[k];
+    l.bytes[k] = (a.copy[k] ? a.head_dim : 2 * a.half) * size;
+    if (v.heads > 0 && (l.bytes[k] != a.head_dim * size || v.head_stride != a.head_dim || v.out_head_stride != a.head_dim)) l.flat = 0;
+  }
+  if (l.flat) l.pitch = a.head_dim * size;
+  l.stage = (l.per * l.pitch + 15) / 16 * 16;
+  // The widest word that every address and length is a multiple of.
+  uintptr_t all = 0;
+  int batches = 0;
+  for (int k = 0; k < 2; ++k) {
+    const g4m_rope_view& v = a.v[k];
+    l.batches[k] = (v.heads + l.per - 1) / l.per;
+    batches += l.batches[k];
+    if (v.heads == 0) continue;
+    all |= (uintptr_t)v.x | (uintptr_t)v.out | (uintptr_t)(v.token_stride * size) | (uintptr_t)(v.out_token_stride * size);
+    if (l.flat) all |= (uintptr_t)(v.heads >= l.per ? l.per * l.pitch : 0) | (uintptr_t)(v.heads % l.per * l.pitch);
+    else all |= (uintptr_t)l.bytes[k] | (uintptr_t)(v.head_stride * size) | (uintptr_t)(v.out_head_stride * size);
+  }
+  l.word = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+  for (int k = 0; k < 2; ++k) l.by_words[k] = fast_div((uint32_t)(l.bytes[k] / l.word));
+  l.by_half = fast_div((uint32_t)a.half);
+  l.by_batches = fast_div((uint32_t)batches);
+  const int threads = l.pitch > 2048 ? 128 : 256, warps = threads / 32;  // at most 32 KB of stages
+  const long want = (long)sms * 6;
+  long tb = std::max<long>(1, std::min<long>(a.tokens / want, 8));
+  tb = std::min<long>(tb, std::max<long>(1, 1024 / a.half));  // and 8 KB of table
+  l.token_block = (int)tb;
+  const long groups = (a.tokens + tb - 1) / tb;
+  const long slices = std::max<long>(1, std::min<long>((tb * batches + warps - 1) / warps, want / groups));
+  const dim3 grid((unsigned)groups, (unsigned)slices);
+  const size_t smem = (size_t)(tb * a.half + 1) / 2 * 16 + (size_t)warps * 2 * l.stage;
+  if (l.word == 16) launch_staged_w<T, 16>(l, grid, threads, smem, st);
+  else if (l.word == 8) launch_staged_w<T, 8>(l, grid, threads, smem, st);
+  else if (l.word == 4) launch_staged_w<T, 4>(l, grid, threads, smem, st);
+  else if (size == 2) launch_staged_w<T, size == 2 ? 2 : 4>(l, grid, threads, smem, st);
+}
+
+template <class T>
+static void launch_rope(const RopeArgs& a, int sms, cudaStream_t st) {
+  if (a.vec) launch_chunks<T>(a, sms, st);
+  else launch_staged<T>(a, sms, st);
+}
+
+cudaError_t rope_run(const RopeArgs& a, int dev, cudaStream_t st) {
+  const int sms = g_num_sms(dev);
+  if (a.dtype == G4M_F32) launch_rope<float>(a, sms, st);
+  else if (a.dtype == G4M_BF16) launch_rope<__nv_bfloat16>(a, sms, st);
+  else launch_rope<__half>(a, sms, st);
   return cudaGetLastError();
 }
 

@@ -417,7 +417,8 @@ def assert_rope(got, exp, mag, dtype, pmax):
 
 @pytest.mark.parametrize("tokens,hq,hk,hd,rotary", [(1, 8, 1, 256, 256), (1, 1, 0, 2, 2), (3, 4, 2, 64, 32), (5, 3, 1, 80, 36),
                                                     (77, 12, 12, 64, 64), (130, 5, 2, 96, 16), (1021, 2, 1, 40, 40), (9, 70, 3, 128, 64),
-                                                    (2, 1, 1, 1024, 1024), (700, 16, 4, 128, 128), (33, 3, 3, 66, 34), (64, 6, 2, 72, 48)])
+                                                    (2, 1, 1, 1024, 1024), (700, 16, 4, 128, 128), (33, 3, 3, 66, 34), (64, 6, 2, 72, 48), (61, 4, 4, 33, 32), (40, 3, 3, 302, 302),
+                                                    (25, 1, 2, 127, 2), (3, 9, 5, 1022, 1022), (2500, 4, 1, 30, 30)])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_rope(ctx, native, tokens, hq, hk, hd, rotary, interleaved, dtype):
