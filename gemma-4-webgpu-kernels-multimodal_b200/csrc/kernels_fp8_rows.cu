@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kQuantThreads, 5) fp8_quantize_kernel(const __
   const int lane16 = threadIdx.x & 15;
   const uint32_t stride = gridDim.x * (kQuantThreads / 16);
   uint32_t u = blockIdx.x * (kQuantThreads / 16) + (threadIdx.x >> 4);
-  Raw8<T> x0, x1;
+  Raw8<T, FULL> x0, x1;
   uint32_t row = 0, kb = 0;
   auto fetch = [&](uint32_t unit) {
     row = div_by(unit, blocks);
@@ -43,18 +43,18 @@ __global__ void __launch_bounds__(kQuantThreads, 5) fp8_quantize_kernel(const __
     const int c = (int)kb * kFp8Block + lane16 * 8;
     const int d = unit < a.units ? a.d : 0;  // past the end: zeros, nothing read
     const T* x = static_cast<const T*>(a.x) + (long)row * a.ldx;
-    load_raw8<FULL>(x, c, d, a.vec & 1, x0);
-    if (ACT != G4M_ACT_NONE) load_raw8<FULL>(x + a.d, c, d, a.vec & 2, x1);
+    load_raw8<T, FULL>(x, c, d, x0);
+    if (ACT != G4M_ACT_NONE) load_raw8<T, FULL>(x + a.d, c, d, x1);
   };
   fetch(u);
   // The two half-warps of a warp hold neighbouring blocks and stay together:
   // the warp goes on while its first has a block.
   for (; u - ((threadIdx.x >> 4) & 1) < a.units; u += stride) {
     float v[8];
-    unpack8(x0, v);
+    unpack8<T, FULL>(x0, v);
     if (ACT != G4M_ACT_NONE) {
       float g[8];
-      unpack8(x1, g);
+      unpack8<T, FULL>(x1, g);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = activate<ACT>(v[j], g[j]);
     }
@@ -103,12 +103,9 @@ cudaError_t fp8_quantize(const QuantArgs& a, int dev, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 struct NormKernelArgs {
   g4m_norm_args a;
-  uint32_t vec;  // which row sets start on 16-byte boundaries (bits below)
   float inv_d;
   FastDiv per_gate;
 };
-enum : uint32_t { kVecY = 1, kVecGate = 2, kVecH = 4, kVecHOut = 8, kVecN = 16, kVecPost = 32, kVecPre = 64 };
-
 // Sum over the threads of the row; every thread gets it.  The two sums of a
 // row alternate between two `part`s, so that one barrier each is enough: a
 // part is written again only after the other sum's barrier.
@@ -137,10 +134,10 @@ __device__ __forceinline__ float square_sum(const float (&v)[NCH][8]) {
 
 // v = v * inv * w for the chunk at column c (w null: all ones).
 template <bool FULL>
-__device__ __forceinline__ void scale8(float (&v)[8], float inv, const float* w, int c, int d, bool vec) {
+__device__ __forceinline__ void scale8(float (&v)[8], float inv, const float* w, int c, int d) {
   if (w) {
     float f[8];
-    load8<FULL>(w, c, d, vec, f);
+    load8<FULL>(w, c, d, f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (v[i] * inv) * f[i];
   } else {
@@ -149,58 +146,66 @@ __device__ __forceinline__ void scale8(float (&v)[8], float inv, const float* w,
   }
 }
 
-// Chunks per thread, the most threads of a row, blocks an SM shall hold.
-template <int NCH>
+// The most threads of a row, blocks an SM shall hold.  Shifting chunks into
+// place (rows off 16-byte boundaries) takes registers: those rows get more
+// threads with fewer chunks each, and no loads ahead, but blocks enough.
+template <int NCH, bool FULL>
 struct NormCfg {
-  static constexpr int T = NCH == 4 ? 512 : 256;
-  static constexpr int BLOCKS = NCH == 1 ? 4 : NCH == 2 ? 3 : 1;
+  static constexpr int T = FULL && NCH < 4 ? 256 : 512;
+  static constexpr int BLOCKS = !FULL ? (NCH == 1 ? 2 : 1) : NCH == 1 ? 4 : NCH == 2 ? 3 : 1;
 };
 
 template <class TY, class TH, int NCH, bool FULL>
-__global__ void __launch_bounds__(NormCfg<NCH>::T, NormCfg<NCH>::BLOCKS)
+__global__ void __launch_bounds__(NormCfg<NCH, FULL>::T, NormCfg<NCH, FULL>::BLOCKS)
     norm_residual_kernel(const __grid_constant__ NormKernelArgs p) {
   __shared__ float part[2][16];
   const g4m_norm_args& a = p.a;
   const int T = blockDim.x, t = threadIdx.x, d = a.d;
-  Raw8<TY> ry[NCH];
-  Raw8<TH> rh[NCH];
+  Raw8<TY, FULL> ry[NCH];
+  Raw8<TH, FULL> rh[NCH];
   auto fetch_y = [&](long row) {
     const int dd = row < a.rows && a.y ? d : 0;  // past the end: zeros, nothing read
     const TY* y = static_cast<const TY*>(a.y) + row * a.ldy;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) load_raw8<FULL>(y, 8 * (k * T + t), dd, p.vec & kVecY, ry[k]);
+    for (int k = 0; k < NCH; ++k) load_raw8<TY, FULL>(y, 8 * (k * T + t), dd, ry[k]);
   };
   auto fetch_h = [&](long row) {
     const int dd = row < a.rows && a.h ? d : 0;
     const TH* x = static_cast<const TH*>(a.h) + row * a.ldh;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) load_raw8<FULL>(x, 8 * (k * T + t), dd, p.vec & kVecH, rh[k]);
+    for (int k = 0; k < NCH; ++k) load_raw8<TH, FULL>(x, 8 * (k * T + t), dd, rh[k]);
   };
   // Rows of one warp share a block four at a time and meet no block barrier.
   const long stride = (long)gridDim.x * blockDim.y;
   long row = (long)blockIdx.x * blockDim.y + threadIdx.y;
-  fetch_y(row);
-  fetch_h(row);
+  if (FULL) {
+    fetch_y(row);
+    fetch_h(row);
+  }
   for (; row < a.rows; row += stride) {
+    if (!FULL) {
+      fetch_y(row);
+      fetch_h(row);
+    }
     float b[NCH][8], h[NCH][8];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      unpack8(ry[k], b[k]);
-      unpack8(rh[k], h[k]);
+      unpack8<TY, FULL>(ry[k], b[k]);
+      unpack8<TH, FULL>(rh[k], h[k]);
     }
-    fetch_y(row + stride);
+    if (FULL) fetch_y(row + stride);
     if (a.y) {
       if (a.norm_post) {
         const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(b), part[0]), p.inv_d, a.eps));
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) scale8<FULL>(b[k], inv, a.w_post, 8 * (k * T + t), d, p.vec & kVecPost);
+        for (int k = 0; k < NCH; ++k) scale8<FULL>(b[k], inv, a.w_post, 8 * (k * T + t), d);
       }
       if (a.gate) {
         const TY* g = static_cast<const TY*>(a.gate) + (long)div_by((uint32_t)row, p.per_gate) * a.ldg;
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
           float f[8];
-          load8<FULL>(g, 8 * (k * T + t), d, p.vec & kVecGate, f);
+          load8<FULL>(g, 8 * (k * T + t), d, f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) b[k][i] *= f[i];
         }
@@ -213,19 +218,19 @@ __global__ void __launch_bounds__(NormCfg<NCH>::T, NormCfg<NCH>::BLOCKS)
     if (a.h_out) {
       TH* o = static_cast<TH*>(a.h_out) + row * a.ldh_out;
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) store8<FULL>(o, 8 * (k * T + t), d, p.vec & kVecHOut, h[k]);
+      for (int k = 0; k < NCH; ++k) store8<FULL>(o, 8 * (k * T + t), d, h[k]);
     }
-    fetch_h(row + stride);  // here, where the branch's registers are free again
+    if (FULL) fetch_h(row + stride);  // here, where the branch's registers are free again
     if (!a.n_out && !a.out.codes) continue;
     if (a.norm_pre) {
       const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(h), part[1]), p.inv_d, a.eps));
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) scale8<FULL>(h[k], inv, a.w_pre, 8 * (k * T + t), d, p.vec & kVecPre);
+      for (int k = 0; k < NCH; ++k) scale8<FULL>(h[k], inv, a.w_pre, 8 * (k * T + t), d);
     }
     if (a.n_out) {
       TY* o = static_cast<TY*>(a.n_out) + row * a.ldn;
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) store8<FULL>(o, 8 * (k * T + t), d, p.vec & kVecN, h[k]);
+      for (int k = 0; k < NCH; ++k) store8<FULL>(o, 8 * (k * T + t), d, h[k]);
     }
     if (a.out.codes) {
       uint8_t* codes = a.out.codes + row * a.out.ldc;
@@ -242,30 +247,37 @@ __global__ void __launch_bounds__(NormCfg<NCH>::T, NormCfg<NCH>::BLOCKS)
   }
 }
 
+// Rows that start on 16-byte boundaries, or are absent.
 static bool rows16(const void* p, int64_t ld, int dtype) {
   const int64_t size = dtype == G4M_F32 ? 4 : 2;
-  return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * size)) % 16 == 0;
+  return !p || (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * size)) % 16 == 0;
 }
 
-template <class TY, class TH, int NCH>
+template <class TY, class TH, int NCH, bool FULL>
 static void launch_norm(const NormKernelArgs& p, int sms, cudaStream_t st) {
+  using C = NormCfg<NCH, FULL>;
   const int chunks = (p.a.d + 7) / 8, T = ((chunks + NCH - 1) / NCH + 31) / 32 * 32;
   const dim3 block(T, T == 32 ? 4 : 1);
   const long blocks = (p.a.rows + block.y - 1) / block.y;
-  const long resident = (long)sms * std::max(1, NormCfg<NCH>::T * NormCfg<NCH>::BLOCKS / (T * (int)block.y));
-  const g4m_norm_args& a = p.a;
-  const bool full = a.d % 8 == 0 && (!a.y || (p.vec & kVecY)) && (!a.gate || (p.vec & kVecGate)) && (!a.h || (p.vec & kVecH)) &&
-                    (!a.h_out || (p.vec & kVecHOut)) && (!a.n_out || (p.vec & kVecN)) && (!a.w_post || (p.vec & kVecPost)) &&
-                    (!a.w_pre || (p.vec & kVecPre));
-  if (full) norm_residual_kernel<TY, TH, NCH, true><<<(unsigned)std::min(blocks, resident), block, 0, st>>>(p);
-  else norm_residual_kernel<TY, TH, NCH, false><<<(unsigned)std::min(blocks, resident), block, 0, st>>>(p);
+  const long resident = (long)sms * std::max(1, C::T * C::BLOCKS / (T * (int)block.y));
+  norm_residual_kernel<TY, TH, NCH, FULL><<<(unsigned)(FULL ? std::min(blocks, resident) : blocks), block, 0, st>>>(p);
 }
 template <class TY, class TH>
 static void launch_norm_h(const NormKernelArgs& p, int sms, cudaStream_t st) {
-  const int chunks = (p.a.d + 7) / 8;
-  if (chunks <= 256) launch_norm<TY, TH, 1>(p, sms, st);
-  else if (chunks <= 512) launch_norm<TY, TH, 2>(p, sms, st);
-  else launch_norm<TY, TH, 4>(p, sms, st);
+  const g4m_norm_args& a = p.a;
+  const int chunks = (a.d + 7) / 8;
+  const bool full = a.d % 8 == 0 && rows16(a.y, a.ldy, a.dtype) && rows16(a.gate, a.ldg, a.dtype) && rows16(a.h, a.ldh, a.h_dtype) &&
+                    rows16(a.h_out, a.ldh_out, a.h_dtype) && rows16(a.n_out, a.ldn, a.dtype) && rows16(a.w_post, 0, G4M_F32) &&
+                    rows16(a.w_pre, 0, G4M_F32);
+  if (full) {
+    if (chunks <= 256) launch_norm<TY, TH, 1, true>(p, sms, st);
+    else if (chunks <= 512) launch_norm<TY, TH, 2, true>(p, sms, st);
+    else launch_norm<TY, TH, 4, true>(p, sms, st);
+  } else {
+    if (chunks <= 512) launch_norm<TY, TH, 1, false>(p, sms, st);
+    else if (chunks <= 1024) launch_norm<TY, TH, 2, false>(p, sms, st);
+    else launch_norm<TY, TH, 4, false>(p, sms, st);
+  }
 }
 template <class TY>
 static void launch_norm_y(const NormKernelArgs& p, int sms, cudaStream_t st) {
@@ -277,10 +289,6 @@ static void launch_norm_y(const NormKernelArgs& p, int sms, cudaStream_t st) {
 cudaError_t norm_residual(const g4m_norm_args& a, int dev, cudaStream_t st) {
   NormKernelArgs p;
   p.a = a;
-  p.vec = (rows16(a.y, a.ldy, a.dtype) ? kVecY : 0) | (rows16(a.gate, a.ldg, a.dtype) ? kVecGate : 0) |
-          (rows16(a.h, a.ldh, a.h_dtype) ? kVecH : 0) | (rows16(a.h_out, a.ldh_out, a.h_dtype) ? kVecHOut : 0) |
-          (rows16(a.n_out, a.ldn, a.dtype) ? kVecN : 0) | (rows16(a.w_post, 0, G4M_F32) ? kVecPost : 0) |
-          (rows16(a.w_pre, 0, G4M_F32) ? kVecPre : 0);
   p.inv_d = 1.0f / (float)a.d;
   p.per_gate = fast_div((uint32_t)std::min<int64_t>(std::max<int64_t>(a.rows_per_gate, 1), 0x7fffffff));
   const int sms = g_num_sms(dev);

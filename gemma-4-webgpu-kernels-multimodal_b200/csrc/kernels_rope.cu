@@ -33,29 +33,29 @@ struct RopeLaunch {
 // [c, c + 8) at columns c and half + c.  Interleaved: columns [2 c, 2 c + 16).
 template <class T, bool INTERLEAVED>
 struct RopeChunk {
-  Raw8<T> p, q;
+  Raw8<T, true> p, q;
   __device__ __forceinline__ void load(const T* x, int c, int half) {
     const int cp = INTERLEAVED ? 2 * c : c, cq = INTERLEAVED ? 2 * c + 8 : half + c;
-    load_raw8(x, cp, cp + 8, true, p);
-    load_raw8(x, cq, cq + 8, true, q);
+    load_raw8<T, true>(x, cp, cp + 8, p);
+    load_raw8<T, true>(x, cq, cq + 8, q);
   }
   __device__ __forceinline__ void turn(T* o, int c, int half, const float2 (&r)[8]) const {
     float a[8], b[8];
-    unpack8(p, a);
-    unpack8(q, b);
+    unpack8<T, true>(p, a);
+    unpack8<T, true>(q, b);
     if (INTERLEAVED) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         turn1(a[2 * i], a[2 * i + 1], r[i]);
         turn1(b[2 * i], b[2 * i + 1], r[4 + i]);
       }
-      store8(o, 2 * c, 2 * c + 8, true, a);
-      store8(o, 2 * c + 8, 2 * c + 16, true, b);
+      store8<true>(o, 2 * c, 2 * c + 8, a);
+      store8<true>(o, 2 * c + 8, 2 * c + 16, b);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) turn1(a[i], b[i], r[i]);
-      store8(o, c, c + 8, true, a);
-      store8(o, half + c, half + c + 8, true, b);
+      store8<true>(o, c, c + 8, a);
+      store8<true>(o, half + c, half + c + 8, b);
     }
   }
   static __device__ __forceinline__ void turn1(float& u, float& v, const float2& r) {
@@ -144,10 +144,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
       for (int h = h0; h < heads; h += step) {
         if (!a.copy[head_of(h, x, o)]) continue;
         if (e + 8 <= a.head_dim) {
-          Raw8<T> r;
-          load_raw8(x, e, e + 8, true, r);
+          Raw8<T, true> r;
+          load_raw8<T, true>(x, e, e + 8, r);
 #pragma unroll
-          for (int i = 0; i < Raw8<T>::WORDS; ++i) reinterpret_cast<uint4*>(o + e)[i] = r.w[i];
+          for (int i = 0; i < Raw8<T, true>::WORDS; ++i) reinterpret_cast<uint4*>(o + e)[i] = r.w[i];
         } else {
           for (int i = e; i < a.head_dim; ++i) o[i] = x[i];
         }
