@@ -119,6 +119,7 @@ int g4m_fp8_quantize(g4m_ctx* ctx, int di, int act, const void* x, int dtype, in
     if (act < G4M_ACT_NONE || act > G4M_ACT_GELU_TANH) return fail(G4M_E_ARG, "unknown activation " + std::to_string(act));
     if (!dtype_ok(dtype)) return fail(G4M_E_ARG, "unknown dtype " + std::to_string(dtype));
     if (rows < 0 || cols <= 0) return fail(G4M_E_ARG, "rows must not be negative and d must be positive");
+    if (cols > kFp8MaxCols) return fail(G4M_E_UNSUPPORTED, "d = " + std::to_string(cols) + " is above " + std::to_string(kFp8MaxCols));
     QuantArgs a;
     a.blocks = (cols - 1) / kFp8Block + 1;
     if (rows > INT_MAX / a.blocks) return fail(G4M_E_UNSUPPORTED, "more than 2^31 - 1 blocks of 128 columns in one call");
@@ -138,7 +139,7 @@ int g4m_fp8_quantize(g4m_ctx* ctx, int di, int act, const void* x, int dtype, in
     a.act = act;
     a.dtype = dtype;
     const int64_t size = dtype_size(dtype);
-    a.vec = (rows16(x, ldx, size) ? 1 : 0) | (rows16((const char*)x + cols * size, ldx, size) ? 2 : 0);
+    a.full = cols % 8 == 0 && rows16(x, ldx, size) && (act == G4M_ACT_NONE || rows16((const char*)x + cols * size, ldx, size));
     a.codes = out->codes;
     a.ldc = out->ldc;
     a.scales = out->scales;
@@ -176,6 +177,8 @@ int g4m_fp8_linear_prepare(g4m_ctx* ctx, int di, const uint8_t* w, const float* 
                            const float* bias, g4m_fp8_linear** out_linear) {
   return no_throw([&]() -> int {
     if (!device_ok(ctx, di) || !w || !w_scales || !out_linear || in <= 0 || out <= 0) return fail(G4M_E_ARG, "bad argument");
+    if (in > kFp8MaxCols || out > kFp8MaxCols)
+      return fail(G4M_E_UNSUPPORTED, "in or out is above " + std::to_string(kFp8MaxCols));
     Device& d = *ctx->devs[di];
     DeviceGuard guard(d.id);
     g4m_fp8_linear* L = new g4m_fp8_linear();

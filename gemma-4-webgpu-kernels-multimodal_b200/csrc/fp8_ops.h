@@ -8,13 +8,15 @@
 
 namespace g4m {
 
+constexpr int kFp8MaxCols = 1 << 24;  // keeps column arithmetic far inside 32 bits
 constexpr int kFp8Block = 128;  // columns of a row (and rows of a weight block) that share one scale
 
 struct QuantArgs {
   const void* x;
   long ldx;
   uint32_t units;  // rows * blocks
-  int d, blocks, act, dtype, vec;
+  int d, blocks, act, dtype;
+  int full;               // rows (both halves) start on 16-byte boundaries and hold whole chunks of 8
   uint8_t* codes;
   long ldc;
   float* scales;

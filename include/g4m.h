@@ -124,7 +124,10 @@ G4M_API int g4m_linear_run_noalloc(g4m_linear* lin, const float* x_dev, int rows
  * width, any alignment; pointers need the alignment of their element type
  * (G4M_E_ARG otherwise), 16-byte aligned rows are faster.  Zero rows are
  * G4M_OK and launch nothing.  Nothing outside the stated rows and columns is
- * written.  Inputs and outputs must not overlap except where stated. */
+ * read or written.  Inputs and outputs must not overlap except where stated.
+ * All are inference operators: none has a backward form.  A device-side wait
+ * that expires shows as G4M_E_TIMEOUT in the next call that waits for the
+ * device (as with g4m_linear_run). */
 
 enum g4m_dtype { G4M_F32 = 0, G4M_BF16 = 1, G4M_F16 = 2 };
 
@@ -149,13 +152,15 @@ enum g4m_act {
 };
 
 /* Quantise v (see g4m_act; computed in f32) into out's rows x d codes and
- * scales.  d >= 1, any value. */
+ * scales.  1 <= d <= 2^24 (G4M_E_UNSUPPORTED above). */
 G4M_API int g4m_fp8_quantize(g4m_ctx* ctx, int device_index, int act, const void* x, int dtype, int64_t ldx, int64_t rows,
                              int d, const g4m_fp8_rows* out, void* stream);
 
 /* Resident 8-bit float linear.  w: e4m3 codes [out][in]; w_scales: f32
  * [ceil(out/128)][ceil(in/128)], one per 128 x 128 block; bias: f32 [out] or
- * NULL; host pointers.  Free a linear before its context is destroyed. */
+ * NULL; host pointers.  in and out are at most 2^24.  Free a linear before its
+ * context is destroyed, and after the last replay of a graph that holds its
+ * calls. */
 typedef struct g4m_fp8_linear g4m_fp8_linear;
 G4M_API int g4m_fp8_linear_prepare(g4m_ctx* ctx, int device_index, const uint8_t* w, const float* w_scales, int out, int in,
                                    const float* bias, g4m_fp8_linear** out_linear);

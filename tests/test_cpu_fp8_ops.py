@@ -21,7 +21,7 @@ def quantize(native, act=0, x=P, dtype=1, ldx=256, rows=4, d=200, codes=P, ldc=2
     (dict(act=1), SHAPE, "stride"), (dict(codes=P + 8), ARG, "16-byte"), (dict(ldc=204), ARG, "16-byte"),
     (dict(ldc=192), SHAPE, "stride"), (dict(scales=P + 2), ARG, "scales"), (dict(codes=None), ARG, "null"),
     (dict(scales=None), ARG, "null"), (dict(lds=3), SHAPE, "scales stride"),
-    (dict(rows=1 << 30, lds=1 << 30), UNSUPPORTED, "blocks"), (dict(), ARG, "context"), (dict(rows=0, x=None), ARG, "context"),
+    (dict(rows=1 << 30, lds=1 << 30), UNSUPPORTED, "blocks"), (dict(d=(1 << 24) + 1, ldx=1 << 25, ldc=1 << 25), UNSUPPORTED, "above"), (dict(), ARG, "context"), (dict(rows=0, x=None), ARG, "context"),
 ])
 def test_quantize_refuses(native, bad, status, says):
     assert quantize(native, **bad) == status

@@ -312,7 +312,8 @@ def run_linear(ctx, c, wc, sw, bias, dtype, pad=0, off=0, st=None):
 SHAPES = [(1, 1, 1), (1, 128, 128), (2, 100, 37), (1, 1536, 6144), (3, 129, 257), (8, 2048, 1000), (15, 640, 255), (16, 768, 2304),
           (17, 768, 300), (31, 4000, 500), (33, 96, 1030), (64, 1024, 512), (65, 257, 129), (100, 512, 777), (127, 384, 640),
           (128, 1536, 1536), (129, 1024, 1537), (200, 130, 2050), (256, 4096, 256), (300, 1100, 1300), (511, 640, 384),
-          (513, 768, 3000), (1000, 500, 999), (2304, 768, 2304), (4100, 1024, 520)]
+          (513, 768, 3000), (1000, 500, 999), (2304, 768, 2304), (4100, 1024, 520), (1, 5000, 11000), (300, 9000, 1300),
+          (600, 4500, 2600), (40, 260, 20000)]
 
 
 @pytest.mark.parametrize("rows,i,o", SHAPES)
