@@ -661,6 +661,79 @@ def test_graphs_and_streams(ctx, native):
         assert torch.equal(layer.qkv, w[2])
 
 
+def test_offsets_past_32_bits(ctx, native):
+    """Three rows each, spread over more than 4 GiB of input and of output."""
+    a, b = (torch.empty(5_400_000_000, dtype=torch.uint8, device="cuda") for _ in range(2))
+    d, rows, ld = 200, 3, 1_200_000_000
+    x = a.view(torch.float16)[:2 * ld + d]
+    pick = lambda t, stride, n: torch.stack([t[r * stride:r * stride + n] for r in range(rows)])  # noqa: E731
+    g = gen(8)
+    for r in range(rows):
+        x[r * ld:r * ld + d] = torch.randn(d, device="cuda", generator=g).half()
+    xs = pick(x, ld, d).clone()
+    # quantise: codes 2.2e9 bytes apart, then the linear reads them there and writes rows 6e8 floats apart
+    ldc = 2_200_000_000
+    scales = torch.empty(2, rows, device="cuda")
+    ctx.fp8_quantize(x.data_ptr(), 2, ld, rows, d, b.data_ptr(), ldc, scales.data_ptr(), rows, stream=stream())
+    small = Codes(rows, d)
+    ctx.fp8_quantize(xs.data_ptr(), 2, d, rows, d, *small.args, stream=stream())
+    assert torch.equal(pick(b, ldc, d), small.buf[:rows, :d]) and torch.equal(scales, small.scales())
+    _, wc, sw, _ = linear_case(rows, d, 300, 3)
+    want = run_linear(ctx, small, wc, sw, None, "f32")
+    lin = ctx.fp8_linear(wc.view(torch.uint8).cpu().numpy(), sw.cpu().numpy())
+    y, ldy = a.view(torch.float32), 600_000_000
+    lin.run(b.data_ptr(), ldc, scales.data_ptr(), rows, rows, y.data_ptr(), 0, ldy, stream=stream())
+    assert torch.equal(pick(y, ldy, 300), want)
+    lin.close()
+    # norm and rotary positions, in place
+    for r in range(rows):
+        x[r * ld:r * ld + d] = xs[r]
+    args = dict(rows=rows, d=d, dtype=2, h_dtype=2, eps=1e-6, norm_pre=1)
+    ctx.norm_residual(native.norm_args(**args, h=x.data_ptr(), ldh=ld, n_out=b.data_ptr(), ldn=ld), stream=stream())
+    n = torch.empty_like(xs)
+    ctx.norm_residual(native.norm_args(**args, h=xs.data_ptr(), ldh=d, n_out=n.data_ptr(), ldn=d), stream=stream())
+    assert torch.equal(pick(b.view(torch.float16), ld, d), n)
+    pos = torch.tensor([5, 70000, 9], device="cuda")
+    for rotary in (200, 48, 34):
+        rope = ctx.rope(d, np.linspace(1, 0.01, rotary // 2))
+        for t, stride in ((x, ld), (xs.view(-1), d)):
+            rope.run(native.rope_view(t.data_ptr(), stride, d, t.data_ptr(), stride, d, 1), None, 2, rows, pos.data_ptr(), stream=stream())
+        assert torch.equal(pick(x, ld, d), xs)
+        rope.close()
+
+
+def test_two_host_threads(ctx, native):
+    """One linear, called from two threads on streams of their own."""
+    import threading
+    layers = [Layer(ctx, native, 20, 5), Layer(ctx, native, 300, 6)]
+    layers[1].weights = layers[0].weights
+    want = []
+    for layer in layers:
+        layer.run()
+        torch.cuda.synchronize()
+        want.append(layer.outputs())
+    failed = []
+
+    def work(layer, exp):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(50):
+                    layer.run()
+                s.synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(layer.outputs(), exp)):
+                    failed.append("outputs differ")
+        except Exception as e:  # a thread's exception would be lost
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(layers, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
 def test_default_stream_is_the_legacy_one(ctx):
     """Stream 0 orders with torch's default stream."""
     x = torch.zeros(64, 4096, device="cuda")
