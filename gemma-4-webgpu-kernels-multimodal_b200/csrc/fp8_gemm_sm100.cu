@@ -292,45 +292,47 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       }
     }
     if (warp >= 2) {
-      // Scale products of one output block (half of the tile): slot it % 4
+      // Scale products of one output block (half of the tile): slot it % 2
       // takes sx[row] * sw for the 128 rows once the epilogue is done with
-      // block it - 2 (so with it - 4, the slot's last).  Loads run two blocks
-      // ahead.  In the epilogue's own threads these loads and their
+      // block it - 2, the slot's last.  Loads run two blocks ahead, into the
+      // next tile, too.  In the epilogue's own threads these loads and their
       // bookkeeping took 200 cycles of every block.
       const int half = warp - 2;
-      uint32_t it = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        int mb, nb;
-        tile_of(tile, tiles_m, tiles_n, mb, nb);
-        const float* sw = a.sw + (long)min(2 * nb + half, oblocks - 1) * kblocks;
-        const float* sx[4];
+      const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+      const long total = (long)mine * kblocks;
+      int tile = blockIdx.x, kb = 0;  // what is fetched next
+      const float *sw = nullptr, *sx[4] = {};
+      float x[2][4], w[2];
+      auto fetch = [&](int to) {
+        if (kb == 0) {
+          int mb, nb;
+          tile_of(min(tile, tiles - 1), tiles_m, tiles_n, mb, nb);
+          sw = a.sw + (long)min(2 * nb + half, oblocks - 1) * kblocks;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sx[j] = a.sx + min((long)mb * C::BM + 32 * j + lane, a.rows - 1);
-        float x[2][4], w[2];
-        auto fetch = [&](int kb, int to) {
-          const int k = min(kb, kblocks - 1);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[to][j] = __ldg(sx[j] + (long)k * a.lds);
-          w[to] = __ldg(sw + k);
-        };
-        auto put = [&](int kb, int from) {
-          if (!warp_wait(&bar_acce[it & 1], ((it >> 1) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag)) return false;
-          float* to = scales + (it % C::SCALE_SLOTS) * 2 * C::BM + half * C::BM + lane;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) to[32 * j] = x[from][j] * w[from];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_scale[it % C::SCALE_SLOTS]);
-          ++it;
-          fetch(kb + 2, from);
-          return true;
-        };
-        fetch(0, 0);
-        fetch(1, 1);
-        for (int kb = 0; kb < kblocks && ok; kb += 2) {
-          ok = put(kb, 0);
-          if (ok && kb + 1 < kblocks) ok = put(kb + 1, 1);
+          for (int j = 0; j < 4; ++j) sx[j] = a.sx + min((long)mb * C::BM + 32 * j + lane, a.rows - 1);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[to][j] = __ldg(sx[j] + (long)kb * a.lds);
+        w[to] = __ldg(sw + kb);
+        if (++kb == kblocks) kb = 0, tile += gridDim.x;
+      };
+      uint32_t it = 0;
+      auto put = [&](int from) {
+        if (!warp_wait(&bar_acce[it & 1], ((it >> 1) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag)) return false;
+        float* to = scales + (it % C::SCALE_SLOTS) * 2 * C::BM + half * C::BM + lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[32 * j] = x[from][j] * w[from];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_scale[it % C::SCALE_SLOTS]);
+        ++it;
+        fetch(from);
+        return true;
+      };
+      fetch(0);
+      fetch(1);
+      while (it < total) {
+        if (!put(0)) break;
+        if (it < total && !put(1)) break;
       }
     }
   } else {
