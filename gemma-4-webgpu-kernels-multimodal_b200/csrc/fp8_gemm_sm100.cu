@@ -16,6 +16,17 @@
 //              distributed shared memory in rank order, so nothing depends on
 //              the order of arrival.
 //
+// What bounds them (B200, device time).  Many rows: 8192 x 4096 -> 8192 bf16
+// takes 252 us (2.18 PFLOP/s; 290 us and 1.9 PFLOP/s when repeated until the
+// power cap holds the clock; a bf16 library product of that size would take
+// 332 us at its measured 1.65 PFLOP/s).  The MMAs of a block take 512 cycles;
+// its sums cross to the epilogue and back (issue 130, MMAs and their arrival
+// 600, loads and half of the sums 330, two wake-ups of about 200) in about
+// 1300 with two accumulators to hide them, and the f32 pipe is busy for 330.
+// TMEM holds no third accumulator of 256 columns.  Few rows: 1 x 4096 -> 32768
+// takes 25 us, 5.4 TB/s; below about 20 MB of weights a call is launch, set-up
+// (0.9 us), first bytes (0.8 us) and the cluster's exchange (0.7 us).
+//
 // Every mbarrier wait is bounded; a timeout records an error word and the
 // CTA unwinds.
 #include <algorithm>
@@ -193,7 +204,7 @@ struct ManyCfg {
   // rounding up.
   static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * EPI_STAGE + SCALE_BYTES + 8 * BARS + 16;
   static_assert(SMEM <= 232448, "over 227 KB of shared memory");
-  static constexpr int GROUP_M = 16;      // row blocks that share the output blocks in L2
+  static constexpr int GROUP_M = 16;  // row blocks that share the output blocks in L2 (4 to 32 take the same time)
 };
 
 __device__ __forceinline__ void tile_of(int tile, int tiles_m, int tiles_n, int& mb, int& nb) {

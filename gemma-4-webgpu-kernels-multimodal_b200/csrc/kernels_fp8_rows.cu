@@ -12,7 +12,11 @@ namespace g4m {
 // ---------------------------------------------------------------------------
 // Quantiser.  16 lanes hold one block (8 columns each): the block's largest
 // magnitude is four shuffles, and nothing else crosses lanes.  Half-warps
-// walk the blocks of all rows with the next block's loads in flight.
+// walk the blocks of all rows with the next block's loads in flight.  8192 x
+// 6144 bf16 with gelu (253 MB) takes 50 us, 5.0 TB/s, 0.77 of the measured
+// copy rate; the issue slots are 70 % busy (26 instructions an element: the
+// sigmoid, the largest magnitude, the rounded quotient).  Without a gate half
+// the instructions go and HBM bounds it.
 // ---------------------------------------------------------------------------
 constexpr int kQuantThreads = 256;
 
@@ -99,7 +103,10 @@ cudaError_t fp8_quantize(const QuantArgs& a, int dev, cudaStream_t st) {
 // k < NCH, so 16 consecutive lanes hold one 128-column block and the e4m3
 // scales need no shared memory.  The two means of squares are the only row
 // sums.  Blocks walk the rows with the next row's loads in flight: with one
-// row per block, loads, sums and stores took turns.
+// row per block, loads, sums and stores took turns.  16384 x 4096 (bf16 branch,
+// f32 residual, gate, codes out: 739 MB) takes 159 us, 4.7 TB/s, 0.71 of the
+// measured copy rate; to bf16 rows without gate 6.0 TB/s, 0.92.  Between them
+// stand the shuffles of the sums and block maxima and the rounded quotients.
 // ---------------------------------------------------------------------------
 struct NormKernelArgs {
   g4m_norm_args a;
