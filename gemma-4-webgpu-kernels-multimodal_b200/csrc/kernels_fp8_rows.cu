@@ -113,9 +113,11 @@ struct NormKernelArgs {
   float inv_d;
   FastDiv per_gate;
 };
-// Sum over the threads of the row; every thread gets it.  The two sums of a
-// row alternate between two `part`s, so that one barrier each is enough: a
-// part is written again only after the other sum's barrier.
+// Sum over the threads of the row; every thread gets it.  The sums that a
+// block forms one after another, of one row or of the next, alternate between
+// two `part`s, so that one barrier each is enough: a part is written again
+// only after the other one's barrier, which every warp reaches with its reads
+// of the first behind it.
 __device__ __forceinline__ float row_sum(float v, float* part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -168,6 +170,7 @@ template <class TY, class TH, int NCH, bool FULL>
 __global__ void __launch_bounds__(NormCfg<NCH, FULL>::T, NormCfg<NCH, FULL>::BLOCKS)
     norm_residual_kernel(const __grid_constant__ NormKernelArgs p) {
   __shared__ float part[2][16];
+  int turn = 0;
   const g4m_norm_args& a = p.a;
   const int T = blockDim.x, t = threadIdx.x, d = a.d;
   Raw8<TY, FULL> ry[NCH];
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(NormCfg<NCH, FULL>::T, NormCfg<NCH, FULL>::BLO
     if (FULL) fetch_y(row + stride);
     if (a.y) {
       if (a.norm_post) {
-        const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(b), part[0]), p.inv_d, a.eps));
+        const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(b), part[turn ^= 1]), p.inv_d, a.eps));
 #pragma unroll
         for (int k = 0; k < NCH; ++k) scale8<FULL>(b[k], inv, a.w_post, 8 * (k * T + t), d);
       }
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(NormCfg<NCH, FULL>::T, NormCfg<NCH, FULL>::BLO
     if (FULL) fetch_h(row + stride);  // here, where the branch's registers are free again
     if (!a.n_out && !a.out.codes) continue;
     if (a.norm_pre) {
-      const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(h), part[1]), p.inv_d, a.eps));
+      const float inv = rsqrtf(fmaf(row_sum(square_sum<NCH>(h), part[turn ^= 1]), p.inv_d, a.eps));
 #pragma unroll
       for (int k = 0; k < NCH; ++k) scale8<FULL>(h[k], inv, a.w_pre, 8 * (k * T + t), d);
     }

@@ -242,6 +242,36 @@ def test_norm_options(ctx, native, opts, d):
     run_norm(ctx, native, **{**dict(rows=37, d=d, dtype="bf16", res="bf16", pad=0, off=0, rpg=5, outs="hnc", seed=d), **opts})
 
 
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("d", [256, 1024, 4096, 8192])
+def test_norm_one_sum_many_rows(ctx, native, post, d):
+    """One of the two norms alone over many rows per block: consecutive sums
+    of a block are then those of different rows.  Rows differ by powers of two
+    up to 2^20, so a sum of another row shows."""
+    rows = 20000
+    g = gen(d + post)
+    x = torch.randn(rows, d, device="cuda", generator=g)
+    x *= torch.exp2(torch.randint(-10, 11, (rows, 1), device="cuda", generator=g).float())
+    x = x.bfloat16()
+    out = torch.empty_like(x)
+    a = dict(rows=rows, d=d, dtype=DT["bf16"][0], h_dtype=DT["bf16"][0], eps=0.0)
+    if post:
+        a.update(y=x.data_ptr(), ldy=d, norm_post=1, h_out=out.data_ptr(), ldh_out=d)
+    else:
+        a.update(h=x.data_ptr(), ldh=d, norm_pre=1, n_out=out.data_ptr(), ldn=d)
+    first = None
+    for _ in range(10):
+        out.zero_()
+        ctx.norm_residual(native.norm_args(**a), stream=stream())
+        if first is None:
+            first = out.clone()
+            for r in range(0, rows, 4000):
+                v = x[r:r + 4000].double()
+                exp = v / torch.sqrt(v.square().mean(1, keepdim=True))
+                assert ((out[r:r + 4000].double() - exp).abs() <= (28 * U + H["bf16"] * (1 + 28 * U)) * exp.abs()).all()
+        assert torch.equal(out, first)
+
+
 def test_norm_rows_that_are_not_finite(ctx, native):
     """A row with a NaN or an infinity spoils itself alone; a row of zeros gives zeros (eps keeps the root above zero)."""
     d = 300
