@@ -169,6 +169,20 @@ __device__ __forceinline__ void load8(const T* row, int c, int d, float (&v)[8])
   unpack8<T, FULL>(r, v);
 }
 
+// Those of the eight elements in w whose bit of mask is set.
+__device__ __forceinline__ void store_elements(float* p, const uint32_t (&w)[8], uint32_t mask) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (mask & (1u << i)) p[i] = __uint_as_float(w[i]);
+}
+template <class T>
+__device__ __forceinline__ void store_elements(T* p, const uint32_t (&w)[4], uint32_t mask) {
+  uint16_t* u = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (mask & (1u << i)) u[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+}
+
 // Elements [c, c + 8) of a row of d, each rounded once; nothing from d on.
 // Without FULL the whole warp calls, its lanes at neighbouring chunks: where
 // the row starts m bytes past a 16-byte boundary, a lane writes the aligned
@@ -185,10 +199,8 @@ __device__ __forceinline__ void store8(T* row, int c, int d, const float (&v)[8]
 #pragma unroll
       for (int i = 0; i < N / 4; ++i)
         reinterpret_cast<uint4*>(row + c)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    } else if (!FULL) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < d) from_f32(v[i], row + c + i);
+    } else if (!FULL && c < d) {
+      store_elements(row + c, w, (1u << (d - c)) - 1);
     }
     return;
   }
@@ -207,12 +219,11 @@ __device__ __forceinline__ void store8(T* row, int c, int d, const float (&v)[8]
   // What no aligned word of a lane covers: this chunk's head, unless the lane
   // before wrote it, and its tail, unless this lane did with the next's head.
   const int head = (16 - m) / sizeof(T), tail = 8 - m / sizeof(T);
-  if (!own || lane == 0 || !next) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool covered = own && (i < head ? lane > 0 : i < tail || next);
-      if (c + i < d && !covered) from_f32(v[i], row + c + i);
-    }
+  if (own) {
+    const uint32_t mask = (lane == 0 ? (1u << head) - 1 : 0u) | (next ? 0u : 0x100u - (1u << tail));
+    if (mask) store_elements(row + c, w, mask);
+  } else if (c < d) {
+    store_elements(row + c, w, (1u << (d - c)) - 1);
   }
 }
 
