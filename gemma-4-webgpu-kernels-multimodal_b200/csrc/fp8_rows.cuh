@@ -253,19 +253,18 @@ __device__ __forceinline__ void with_type(int dtype, F f) {
   else f(static_cast<__half*>(nullptr));
 }
 
-// Bits of the largest magnitude of v.  Magnitudes compare as integers, and
-// there infinities and NaN come above every finite value, so a block that
-// holds one keeps it.
-__device__ __forceinline__ uint32_t amax_bits8(const float (&v)[8]) {
-  uint32_t m = 0;
+// Largest magnitude of v; a NaN among them makes it NaN.
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+  float m = fabsf(v[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 1; i < 7; i += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[i])), "f"(fabsf(v[i + 1])));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[7])));
   return m;
 }
 // Over the 16 lanes that hold one block of 128 columns (all 32 lanes call).
-__device__ __forceinline__ uint32_t block_amax_bits(uint32_t m) {
+__device__ __forceinline__ float block_amax(float m) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 8; o > 0; o >>= 1) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__shfl_xor_sync(0xffffffffu, m, o)));
   return m;
 }
 
@@ -280,9 +279,9 @@ __device__ __forceinline__ float div_by_rcp(float n, float d, float r) {
 // scale = max(amax, 2^-96) / 448; the floor keeps the scale of an all-zero
 // block (and its reciprocal) a normal number.  NaN for a block that is not
 // finite.
-__device__ __forceinline__ float fp8_scale(uint32_t amax_bits) {
-  const float s = div_by_rcp(fmaxf(__uint_as_float(amax_bits), 0x1p-96f), 448.0f, 1.0f / 448.0f);
-  return amax_bits < 0x7f800000u ? s : __uint_as_float(0x7fffffffu);
+__device__ __forceinline__ float fp8_scale(float amax) {
+  const float s = div_by_rcp(fmaxf(amax, 0x1p-96f), 448.0f, 1.0f / 448.0f);
+  return amax < __int_as_float(0x7f800000) ? s : __uint_as_float(0x7fffffffu);
 }
 
 // Eight codes e4m3(v / s), to nearest even, of the rounded quotient: the
