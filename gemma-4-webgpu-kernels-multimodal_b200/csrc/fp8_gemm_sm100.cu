@@ -215,9 +215,15 @@ __device__ __forceinline__ void tile_of(int tile, int tiles_m, int tiles_n, int&
   mb = m0 + r - nb * gm;
 }
 
+// Tiles [0, full) go round the CTAs whole.  The rest, fewer than half the SMs,
+// are cut into 2^lg units of 256 >> lg outputs, one for a CTA, its last.
+struct ManySplit {
+  int full, lg;
+};
+
 __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
     fp8_gemm_many_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap my,
-                         const __grid_constant__ Fp8GemmArgs a) {
+                         const __grid_constant__ Fp8GemmArgs a, const ManySplit cut) {
   using C = ManyCfg;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
@@ -233,6 +239,17 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kblocks = (a.in + kFp8Block - 1) / kFp8Block, oblocks = (a.out + kFp8Block - 1) / kFp8Block;
   const int tiles_m = (int)((a.rows + C::BM - 1) / C::BM), tiles_n = (oblocks + 1) / 2, tiles = tiles_m * tiles_n;
+  // This CTA's share: whole tiles blockIdx.x, + gridDim.x, ..., then maybe a unit.
+  const int whole = cut.full > (int)blockIdx.x ? (cut.full - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  const bool unit = (int)blockIdx.x < (tiles - cut.full) << cut.lg;
+  const int share = whole + unit, width = C::BN >> cut.lg;
+  // Row block, and first output, of the i-th of the share.
+  auto place_of = [&](int i, int& mb, int& col) {
+    const bool cutup = i >= whole;
+    int nb;
+    tile_of(cutup ? cut.full + ((int)blockIdx.x >> cut.lg) : (int)blockIdx.x + i * (int)gridDim.x, tiles_m, tiles_n, mb, nb);
+    col = nb * C::BN + (cutup ? ((int)blockIdx.x & ((1 << cut.lg) - 1)) * width : 0);
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -256,10 +273,12 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
     if (warp == 0 && lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        int mb, nb;
-        tile_of(tile, tiles_m, tiles_n, mb, nb);
-        const uint8_t* w = a.w + (long)2 * nb * kblocks * kFp8TileBytes;
+      for (int i = 0; i < share && ok; ++i) {
+        int mb, col;
+        place_of(i, mb, col);
+        const uint8_t* w = a.w + (long)(col / kFp8Block) * kblocks * kFp8TileBytes + col % kFp8Block * 128;
+        const bool two = i < whole;  // both output blocks, or part of one
+        const int bytes = two ? kFp8TileBytes : width * 128;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % C::STAGES;
           // An earlier kernel on this device failed: looked up once the first
@@ -270,10 +289,10 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
             break;
           }
           uint8_t* sa = smem + s * C::STAGE_BYTES;
-          mbar_expect_tx(&bar_full[s], C::STAGE_BYTES);
+          mbar_expect_tx(&bar_full[s], C::A_BYTES + (two ? C::B_BYTES : bytes));
           tma_load_2d(sa, &mx, &bar_full[s], kb * kFp8Block, mb * C::BM);
-          bulk_load(sa + C::A_BYTES, w + (long)kb * kFp8TileBytes, kFp8TileBytes, &bar_full[s]);
-          bulk_load(sa + C::A_BYTES + kFp8TileBytes, w + (long)(kblocks + kb) * kFp8TileBytes, kFp8TileBytes, &bar_full[s]);
+          bulk_load(sa + C::A_BYTES, w + (long)kb * kFp8TileBytes, bytes, &bar_full[s]);
+          if (two) bulk_load(sa + C::A_BYTES + kFp8TileBytes, w + (long)(kblocks + kb) * kFp8TileBytes, kFp8TileBytes, &bar_full[s]);
         }
       }
       for (uint32_t j = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; j < it; ++j)
@@ -283,12 +302,13 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       // bar_done of a stage tells both that the stage is free and that the
       // block's sums are complete; the epilogue waits for every one, so no
       // arrival is on its way when the CTA exits.
-      constexpr uint32_t idesc = idesc_e4m3_f32(C::BM, C::BN);
+      const uint32_t wide = idesc_e4m3_f32(C::BM, C::BN), narrow = idesc_e4m3_f32(C::BM, width);
       const uint64_t dbase = desc_k_sw128(smem_u32(smem));
-      const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
-      const long total = (long)mine * kblocks;
+      const long total = (long)share * kblocks;
+      const uint32_t cut_at = (uint32_t)whole * (uint32_t)kblocks;
       uint32_t it = 0;
       bool full = false, free = true;  // tested ahead
+      uint32_t idesc = cut_at ? wide : narrow;
       for (; it < total; ++it) {
         const int s = it % C::STAGES;
         const uint32_t b = it & 1;
@@ -298,6 +318,7 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
           break;
         tc_fence_after();
         mma_block(tmem_base + b * C::BN, da, desc_add(da, C::A_BYTES), idesc, &bar_done[s]);
+        idesc = it + 1 < cut_at ? wide : narrow;
         full = mbar_test(&bar_full[(it + 1) % C::STAGES], ((it + 1) / C::STAGES) & 1);
         free = mbar_test(&bar_acce[b ^ 1], (((it + 1) >> 1) & 1) ^ 1);
       }
@@ -309,23 +330,22 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       // next tile, too.  In the epilogue's own threads these loads and their
       // bookkeeping took 200 cycles of every block.
       const int half = warp - 2;
-      const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
-      const long total = (long)mine * kblocks;
-      int tile = blockIdx.x, kb = 0;  // what is fetched next
+      const long total = (long)share * kblocks;
+      int i = 0, kb = 0;  // what is fetched next
       const float *sw = nullptr, *sx[4] = {};
       float x[2][4], w[2];
       auto fetch = [&](int to) {
         if (kb == 0) {
-          int mb, nb;
-          tile_of(min(tile, tiles - 1), tiles_m, tiles_n, mb, nb);
-          sw = a.sw + (long)min(2 * nb + half, oblocks - 1) * kblocks;
+          int mb, col;
+          place_of(min(i, share - 1), mb, col);
+          sw = a.sw + (long)min(col / kFp8Block + (i < whole ? half : 0), oblocks - 1) * kblocks;
 #pragma unroll
           for (int j = 0; j < 4; ++j) sx[j] = a.sx + min((long)mb * C::BM + 32 * j + lane, a.rows - 1);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[to][j] = __ldg(sx[j] + (long)kb * a.lds);
         w[to] = __ldg(sw + kb);
-        if (++kb == kblocks) kb = 0, tile += gridDim.x;
+        if (++kb == kblocks) kb = 0, ++i;
       };
       uint32_t it = 0;
       auto put = [&](int from) {
@@ -352,22 +372,25 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
     // thread, and one half (one output block) of the tile's columns.
     const int q = warp & 3, half = (warp - 4) >> 2;
     uint8_t* stage = smem + C::STAGES * C::STAGE_BYTES + (warp - 4) * C::EPI_STAGE;
-    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + half * 128;
+    const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16);
     const float* scale = scales + half * C::BM + 32 * q + lane;
     uint32_t it = 0;
     bool ok = true, done = false, scaled = false;  // the next block's barriers, tested ahead
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      int mb, nb;
-      tile_of(tile, tiles_m, tiles_n, mb, nb);
+    // One of the share, COLS columns for this warp.
+    auto complete = [&](int i, auto cols) {
+      constexpr int COLS = decltype(cols)::value;
+      int mb, col0;
+      place_of(i, mb, col0);
       const long row0 = (long)mb * C::BM + 32 * q;
-      const int col0 = nb * C::BN + half * 128;
-      float acc[128];
+      col0 += half * COLS;
+      const uint32_t tm = lanes + half * COLS;
+      float acc[COLS];
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+      for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
       if (a.bias) {  // padded with zeros to whole tiles
         const float4* bp = reinterpret_cast<const float4*>(a.bias + col0);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < COLS / 4; ++i) {
           const float4 f = __ldg(bp + i);
           acc[4 * i] = f.x, acc[4 * i + 1] = f.y, acc[4 * i + 2] = f.z, acc[4 * i + 3] = f.w;
         }
@@ -383,32 +406,34 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         // back to the MMA issuer once the last block is loaded, with half of
         // the sums still to be added.  (Single fma: pairs of f32 in one
         // instruction took 14 % longer here.)
-        uint32_t r[4][16];
+        uint32_t r[4][16] = {};
         auto load = [&](int c) { tmem_ld16(src + 16 * c, r[c & 3]); };
         auto add = [&](int c) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(__uint_as_float(r[c & 3][i]), s, acc[16 * c + i]);
         };
 #pragma unroll
-        for (int c = 0; c < 4; ++c) load(c);
+        for (int c = 0; c < COLS / 16 && c < 4; ++c) load(c);
         tmem_wait64(r);
+        if constexpr (COLS > 64) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          add(c);
-          load(c + 4);
+          for (int c = 0; c < 4; ++c) {
+            add(c);
+            load(c + 4);
+          }
+          tmem_wait64(r);
         }
-        tmem_wait64(r);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_acce[b]);
         done = mbar_test(&bar_done[(it + 1) % C::STAGES], ((it + 1) / C::STAGES) & 1);
         scaled = mbar_test(&bar_scale[(it + 1) % C::SCALE_SLOTS], ((it + 1) / C::SCALE_SLOTS) & 1);
 #pragma unroll
-        for (int c = 4; c < 8; ++c) add(c);
+        for (int c = COLS > 64 ? 4 : 0; c < COLS / 16; ++c) add(c);
       }
-      if (!ok) break;
+      if (!ok) return;
       const int nrows = (int)min(32l, a.rows - row0);
-      if (nrows <= 0 || col0 >= a.out) continue;
+      if (nrows <= 0 || col0 >= a.out) return;
       // 16 columns (f32) or 32 (16 bits) at a time: 64 bytes of each of the
       // warp's 32 rows go through shared memory, 16-byte chunk c of row r at
       // c ^ (r / 2 & 3), and out by TMA while the next ones are packed.
@@ -442,7 +467,7 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       };
       if (a.y_dtype == G4M_F32) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < COLS / 16; ++c) {
           if (col0 + 16 * c >= a.out) break;
           uint4 o[4];
 #pragma unroll
@@ -453,7 +478,7 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         }
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < COLS / 32; ++c) {
           if (col0 + 32 * c >= a.out) break;
           uint4 o[4];
 #pragma unroll
@@ -469,6 +494,11 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
           send(o, col0 + 32 * c, 2);
         }
       }
+    };
+    for (int i = 0; i < whole && ok; ++i) complete(i, std::integral_constant<int, 128>());
+    if (unit && ok) {
+      if (cut.lg == 1) complete(whole, std::integral_constant<int, 64>());
+      else complete(whole, std::integral_constant<int, 32>());
     }
     if (lane == 0) tma_store_wait();
   }
@@ -797,7 +827,12 @@ cudaError_t fp8_gemm(const Fp8GemmArgs& a, int dev, cudaStream_t st) {
   else if (!make_tmap_out(&my, a.y, a.rows, a.out, a.ldy, a.y_dtype == G4M_F32 ? 4 : 2, 32)) return cudaErrorInvalidValue;
   const long tiles = (a.rows + ManyCfg::BM - 1) / ManyCfg::BM * ((fp8_blocks(a.out) + 1) / 2);
   if (tiles > 0x3fffffffL) return cudaErrorInvalidValue;
-  fp8_gemm_many_kernel<<<(unsigned)std::min<long>(tiles, sms), ManyCfg::THREADS, ManyCfg::SMEM, st>>>(mx, my, a);
+  const int rest = (int)(tiles % sms);
+  ManySplit cut;
+  cut.lg = 4 * rest <= sms ? 2 : 2 * rest <= sms ? 1 : 0;
+  cut.full = (int)tiles - (cut.lg ? rest : 0);
+  const int grid = tiles >= sms ? sms : (int)(tiles << cut.lg);
+  fp8_gemm_many_kernel<<<grid, ManyCfg::THREADS, ManyCfg::SMEM, st>>>(mx, my, a, cut);
   return cudaGetLastError();
 }
 
