@@ -215,15 +215,14 @@ __device__ __forceinline__ void tile_of(int tile, int tiles_m, int tiles_n, int&
   mb = m0 + r - nb * gm;
 }
 
-// Tiles [0, full) go round the CTAs whole.  The rest, fewer than half the SMs,
-// are cut into 2^lg units of 256 >> lg outputs, one for a CTA, its last.
-struct ManySplit {
-  int full, lg;
-};
-
+// Tiles [0, full) go round the CTAs whole.  The rest, at most SMs >> LG of
+// them, are cut into 2^LG units of 256 >> LG outputs, one for a CTA, its last.
+// A kernel for each LG: the narrow epilogues beside the wide one cost it 2 to
+// 5 % (8192 x 4096 -> 8192 255 and 261 us).
+template <int LG>
 __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
     fp8_gemm_many_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap my,
-                         const __grid_constant__ Fp8GemmArgs a, const ManySplit cut) {
+                         const __grid_constant__ Fp8GemmArgs a, const int full) {
   using C = ManyCfg;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
@@ -240,15 +239,17 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
   const int kblocks = (a.in + kFp8Block - 1) / kFp8Block, oblocks = (a.out + kFp8Block - 1) / kFp8Block;
   const int tiles_m = (int)((a.rows + C::BM - 1) / C::BM), tiles_n = (oblocks + 1) / 2, tiles = tiles_m * tiles_n;
   // This CTA's share: whole tiles blockIdx.x, + gridDim.x, ..., then maybe a unit.
-  const int whole = cut.full > (int)blockIdx.x ? (cut.full - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-  const bool unit = (int)blockIdx.x < (tiles - cut.full) << cut.lg;
-  const int share = whole + unit, width = C::BN >> cut.lg;
+  const int cta = (int)blockIdx.x, ctas = (int)gridDim.x, last = LG ? full : tiles;
+  const int whole = last > cta ? (last - 1 - cta) / ctas + 1 : 0;
+  const bool unit = LG > 0 && cta < (tiles - full) << LG;
+  const int share = whole + unit;
+  constexpr int WIDTH = C::BN >> LG;
   // Row block, and first output, of the i-th of the share.
   auto place_of = [&](int i, int& mb, int& col) {
-    const bool cutup = i >= whole;
+    const bool cut = LG > 0 && i >= whole;
     int nb;
-    tile_of(cutup ? cut.full + ((int)blockIdx.x >> cut.lg) : (int)blockIdx.x + i * (int)gridDim.x, tiles_m, tiles_n, mb, nb);
-    col = nb * C::BN + (cutup ? ((int)blockIdx.x & ((1 << cut.lg) - 1)) * width : 0);
+    tile_of(cut ? full + (cta >> LG) : cta + i * ctas, tiles_m, tiles_n, mb, nb);
+    col = nb * C::BN + (cut ? (cta & ((1 << LG) - 1)) * WIDTH : 0);
   };
 
   if (threadIdx.x == 0) {
@@ -277,8 +278,8 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         int mb, col;
         place_of(i, mb, col);
         const uint8_t* w = a.w + (long)(col / kFp8Block) * kblocks * kFp8TileBytes + col % kFp8Block * 128;
-        const bool two = i < whole;  // both output blocks, or part of one
-        const int bytes = two ? kFp8TileBytes : width * 128;
+        const bool two = LG == 0 || i < whole;  // both output blocks, or part of one
+        const int bytes = two ? kFp8TileBytes : WIDTH * 128;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % C::STAGES;
           // An earlier kernel on this device failed: looked up once the first
@@ -302,26 +303,26 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       // bar_done of a stage tells both that the stage is free and that the
       // block's sums are complete; the epilogue waits for every one, so no
       // arrival is on its way when the CTA exits.
-      const uint32_t wide = idesc_e4m3_f32(C::BM, C::BN), narrow = idesc_e4m3_f32(C::BM, width);
       const uint64_t dbase = desc_k_sw128(smem_u32(smem));
-      const long total = (long)share * kblocks;
-      const uint32_t cut_at = (uint32_t)whole * (uint32_t)kblocks;
       uint32_t it = 0;
       bool full = false, free = true;  // tested ahead
-      uint32_t idesc = cut_at ? wide : narrow;
-      for (; it < total; ++it) {
-        const int s = it % C::STAGES;
-        const uint32_t b = it & 1;
-        const uint64_t da = desc_add(dbase, s * C::STAGE_BYTES);
-        if (!warp_wait(full, &bar_full[s], (it / C::STAGES) & 1, a.err, kErrWaitFull, &abort_flag) ||
-            !warp_wait(free, &bar_acce[b], ((it >> 1) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag))
-          break;
-        tc_fence_after();
-        mma_block(tmem_base + b * C::BN, da, desc_add(da, C::A_BYTES), idesc, &bar_done[s]);
-        idesc = it + 1 < cut_at ? wide : narrow;
-        full = mbar_test(&bar_full[(it + 1) % C::STAGES], ((it + 1) / C::STAGES) & 1);
-        free = mbar_test(&bar_acce[b ^ 1], (((it + 1) >> 1) & 1) ^ 1);
-      }
+      auto issue = [&](long until, uint32_t idesc) {
+        for (; it < until; ++it) {
+          const int s = it % C::STAGES;
+          const uint32_t b = it & 1;
+          const uint64_t da = desc_add(dbase, s * C::STAGE_BYTES);
+          if (!warp_wait(full, &bar_full[s], (it / C::STAGES) & 1, a.err, kErrWaitFull, &abort_flag) ||
+              !warp_wait(free, &bar_acce[b], ((it >> 1) & 1) ^ 1, a.err, kErrWaitAccEmpty, &abort_flag))
+            return false;
+          tc_fence_after();
+          mma_block(tmem_base + b * C::BN, da, desc_add(da, C::A_BYTES), idesc, &bar_done[s]);
+          full = mbar_test(&bar_full[(it + 1) % C::STAGES], ((it + 1) / C::STAGES) & 1);
+          free = mbar_test(&bar_acce[b ^ 1], (((it + 1) >> 1) & 1) ^ 1);
+        }
+        return true;
+      };
+      const bool ok = issue((long)whole * kblocks, idesc_e4m3_f32(C::BM, C::BN));
+      if (unit && ok) issue((long)share * kblocks, idesc_e4m3_f32(C::BM, WIDTH));
     }
     if (warp >= 2) {
       // Scale products of one output block (half of the tile): slot it % 2
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         if (kb == 0) {
           int mb, col;
           place_of(min(i, share - 1), mb, col);
-          sw = a.sw + (long)min(col / kFp8Block + (i < whole ? half : 0), oblocks - 1) * kblocks;
+          sw = a.sw + (long)min(col / kFp8Block + (LG == 0 || i < whole ? half : 0), oblocks - 1) * kblocks;
 #pragma unroll
           for (int j = 0; j < 4; ++j) sx[j] = a.sx + min((long)mb * C::BM + 32 * j + lane, a.rows - 1);
         }
@@ -496,9 +497,8 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       }
     };
     for (int i = 0; i < whole && ok; ++i) complete(i, std::integral_constant<int, 128>());
-    if (unit && ok) {
-      if (cut.lg == 1) complete(whole, std::integral_constant<int, 64>());
-      else complete(whole, std::integral_constant<int, 32>());
+    if constexpr (LG > 0) {
+      if (unit && ok) complete(whole, std::integral_constant<int, WIDTH / 2>());
     }
     if (lane == 0) tma_store_wait();
   }
@@ -519,29 +519,26 @@ struct FewCfg {
   static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
   // Two CTAs fit an SM.  (Twice the stages for grids of one CTA per SM gained
   // nothing, and cost half a microsecond a launch.)
-  static constexpr int STAGES = NT == 16 ? 5 : NT == 32 ? 4 : 3;
+  static constexpr int STAGES = NT == 16 ? 5 : 4;
   // One accumulator per stage: bar_done of a stage stands for both, and no
   // wait on it can fall a whole turn behind.
-  static constexpr int TMEM_COLS = STAGES * NT <= 128 ? 128 : 256;
-  // An epilogue warp holds 32 outputs of up to 32 rows: one warpgroup for each
-  // 32 rows (with 64 rows in a warp, a block's sums took 925 cycles).
-  static constexpr int RP = NT < 32 ? NT : 32, GROUPS = NT / RP;
-  static constexpr int SCALE_BLOCKS = NT == 16 ? 8 : NT == 32 ? 4 : 2;  // column blocks whose row scales are fetched together
+  static constexpr int TMEM_COLS = 128;
+  static constexpr int SCALE_BLOCKS = NT == 16 ? 8 : 4;  // column blocks whose row scales are fetched together
   static constexpr int SCALE_BYTES = 4 * 2 * SCALE_BLOCKS * NT * 4;     // per epilogue warp, double-buffered
   static constexpr int PART_BYTES = NT * 128 * 4;  // partial totals from the cluster: splits * ceil(rows / splits) <= NT rows, splits a power of 2
   static constexpr int BARS = 3 * STAGES + 1;
-  static constexpr int THREADS = 64 + 128 * GROUPS;
+  static constexpr int THREADS = 192;
   static constexpr int SMEM = STAGES * STAGE_BYTES + SCALE_BYTES + PART_BYTES + 1024;
+  static_assert(STAGES * NT <= TMEM_COLS, "an accumulator per stage");
   static_assert(NT * 512 <= STAGES * STAGE_BYTES, "the outgoing totals reuse the stages");
   static_assert(2 * TMEM_COLS <= 512 && 2 * (SMEM + 1024 + 512) <= 233472, "over the SM's memories");
 };
 
-// Rows first, first + step, ... of n: the S partial totals, [rank][row][128],
-// added in rank order.
-template <int S, int STEP, class T>
-__device__ __forceinline__ void add_parts(const float* part, int n, int first, float bias, T* y, long ldy) {
+// n rows: the S partial totals, [rank][row][128], added in rank order.
+template <int S, class T>
+__device__ __forceinline__ void add_parts(const float* part, int n, float bias, T* y, long ldy) {
 #pragma unroll 4
-  for (int j = first; j < n; j += STEP) {
+  for (int j = 0; j < n; ++j) {
     float total = part[j * 128];
 #pragma unroll
     for (int p = 1; p < S; ++p) total += part[(p * n + j) * 128];
@@ -575,7 +572,7 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
   // sums are complete.
   uint64_t *bar_full = bars, *bar_done = bars + C::STAGES, *bar_acce = bars + 2 * C::STAGES, *bar_part = bars + C::BARS - 1;
   if (threadIdx.x < C::BARS) {
-    mbar_init(bars + threadIdx.x, bars + threadIdx.x >= bar_acce && bars + threadIdx.x < bar_part ? 4 * C::GROUPS : 1);
+    mbar_init(bars + threadIdx.x, bars + threadIdx.x >= bar_acce && bars + threadIdx.x < bar_part ? 4 : 1);
     fence_mbar_init();
     if (splits > 1 && bars + threadIdx.x == bar_part) mbar_expect_tx(bar_part, (uint32_t)(splits * (j1 - j0) * 512));
     if (threadIdx.x == 0) abort_flag = 0;
@@ -587,11 +584,11 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
   tc_fence_after();
   if (splits > 1) cluster_arrive();  // this CTA's barriers can be reached from the others
   const uint32_t tmem_base = tmem_slot;
-  // Epilogue: output ob * 128 + t, rows r0 .. r0 + RP - 1 of the tile.
-  const int q = warp & 3, t = 32 * q + lane, group = (warp - 2) >> 2, r0 = group * C::RP;
-  uint64_t acc[C::RP / 2];  // row pairs
+  // Epilogue: output ob * 128 + t, all rows of the tile.
+  const int q = warp & 3, t = 32 * q + lane;
+  uint64_t acc[NT / 2];  // row pairs
 #pragma unroll
-  for (int i = 0; i < C::RP / 2; ++i) acc[i] = 0;
+  for (int i = 0; i < NT / 2; ++i) acc[i] = 0;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -624,19 +621,19 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
       mma_block(tmem_base + s * NT, dw, desc_add(dw, C::W_BYTES), idesc, &bar_done[s]);
     }
   } else {
-    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + r0;
+    const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16);
     const float* swp = a.sw + (long)ob * kblocks + k0;
     const float* sxp = a.sx + (long)k0 * a.lds + row0;
     // Row scales come a few column blocks at a time, one fetch ahead; the
     // weight scales of 32 blocks sit in the lanes.
     constexpr int SB = C::SCALE_BLOCKS;
-    float* sc = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + C::PART_BYTES) + (warp - 2) * 2 * SB * C::RP;
+    float* sc = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + C::PART_BYTES) + (warp - 2) * 2 * SB * NT;
     auto fetch = [&](int g) {
 #pragma unroll
-      for (int p = 0; p < SB * C::RP / 32; ++p) {
-        const int e = lane + 32 * p, i = g * SB + e / C::RP, j = r0 + e % C::RP;
+      for (int p = 0; p < SB * NT / 32; ++p) {
+        const int e = lane + 32 * p, i = g * SB + e / NT, j = e % NT;
         const bool valid = i < nk && j < nrows;
-        cp_async4(sc + (g & 1) * SB * C::RP + e, valid ? sxp + (long)i * a.lds + j : sxp, valid);
+        cp_async4(sc + (g & 1) * SB * NT + e, valid ? sxp + (long)i * a.lds + j : sxp, valid);
       }
       cp_async_commit();
     };
@@ -655,16 +652,16 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
       }
       const float w = __shfl_sync(0xffffffffu, wl, i & 31);
       const uint64_t ww = pack_f32x2(w, w);
-      const float* s = sc + (i / SB & 1) * SB * C::RP + i % SB * C::RP;
+      const float* s = sc + (i / SB & 1) * SB * NT + i % SB * NT;
       const int b = i % C::STAGES;
       if (!warp_wait(&bar_done[b], (i / C::STAGES) & 1, a.err, kErrWaitAccFull, &abort_flag)) break;
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < C::RP / 16; ++c) {
+      for (int c = 0; c < NT / 16; ++c) {
         uint32_t r[16];
         tmem_ld16(tm + b * NT + 16 * c, r);
         tmem_wait16(r);
-        if (c == C::RP / 16 - 1) {
+        if (c == NT / 16 - 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_acce[b]);
@@ -685,12 +682,12 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
   if (splits == 1) {
     if (warp >= 2 && o < a.out)
       with_type(a.y_dtype, [&](auto* tp) {
-        auto* y = static_cast<decltype(tp)>(a.y) + (row0 + r0) * a.ldy + o;
+        auto* y = static_cast<decltype(tp)>(a.y) + row0 * a.ldy + o;
 #pragma unroll
-        for (int j = 0; j < C::RP; ++j) {
+        for (int j = 0; j < NT; ++j) {
           float v[2];
           unpack_f32x2(acc[j / 2], v[0], v[1]);
-          if (r0 + j < nrows) from_f32(v[j & 1] + bias, y + j * a.ldy);
+          if (j < nrows) from_f32(v[j & 1] + bias, y + j * a.ldy);
         }
       });
   } else {
@@ -700,15 +697,15 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
     // MMAs are done.
     bool ok = true;
     if (warp >= 2) {
-      float* own = reinterpret_cast<float*>(smem) + r0 * 128 + t;
+      float* own = reinterpret_cast<float*>(smem) + t;
 #pragma unroll
-      for (int j = 0; j < C::RP; ++j) {
+      for (int j = 0; j < NT; ++j) {
         float v[2];
         unpack_f32x2(acc[j / 2], v[0], v[1]);
-        if (r0 + j < nrows) own[j * 128] = v[j & 1];
+        if (j < nrows) own[j * 128] = v[j & 1];
       }
       fence_proxy_async_smem();
-      asm volatile("bar.sync 1, %0;" ::"n"(128 * C::GROUPS) : "memory");
+      asm volatile("bar.sync 1, 128;" ::: "memory");
     }
     cluster_wait();
     if (warp >= 2) {
@@ -723,9 +720,9 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
       if (ok && o < a.out)
         with_type(a.y_dtype, [&](auto* tp) {
           auto* y = static_cast<decltype(tp)>(a.y) + (row0 + j0) * a.ldy + o;
-          if (lg == 1) add_parts<2, C::GROUPS>(part + t, j1 - j0, group, bias, y, a.ldy);
-          else if (lg == 2) add_parts<4, C::GROUPS>(part + t, j1 - j0, group, bias, y, a.ldy);
-          else add_parts<8, C::GROUPS>(part + t, j1 - j0, group, bias, y, a.ldy);
+          if (lg == 1) add_parts<2>(part + t, j1 - j0, bias, y, a.ldy);
+          else if (lg == 2) add_parts<4>(part + t, j1 - j0, bias, y, a.ldy);
+          else add_parts<8>(part + t, j1 - j0, bias, y, a.ldy);
         });
     }
     // No CTA leaves while another one may still push to it.
@@ -774,11 +771,17 @@ static cudaError_t setup_few() {
   return cudaFuncSetAttribute(fp8_gemm_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
 }
 
+template <int LG>
+static cudaError_t setup_many() {
+  return cudaFuncSetAttribute(fp8_gemm_many_kernel<LG>, cudaFuncAttributeMaxDynamicSharedMemorySize, ManyCfg::SMEM);
+}
+
 cudaError_t fp8_gemm_setup() {
-  cudaError_t e = cudaFuncSetAttribute(fp8_gemm_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ManyCfg::SMEM);
+  cudaError_t e = setup_many<0>();
+  if (e == cudaSuccess) e = setup_many<1>();
+  if (e == cudaSuccess) e = setup_many<2>();
   if (e == cudaSuccess) e = setup_few<16>();
   if (e == cudaSuccess) e = setup_few<32>();
-  if (e == cudaSuccess) e = setup_few<64>();
   return e;
 }
 
@@ -791,8 +794,8 @@ static cudaError_t launch_few(const Fp8GemmArgs& a, int sms, cudaStream_t st) {
   // Split the column blocks while the CTAs stay about as many as the SMs and
   // keep four blocks each, or fewer where they would leave most SMs idle.
   // (1 x 4096 -> 4096: 11.7 us unsplit, 8.6 / 7.1 / 8.2 split by 2 / 4 / 8;
-  // 1 x 1536 -> 12288, 96 CTAs unsplit: 7.5, and 8.6 split by 2; 100 x 768 ->
-  // 2304: 5.9, and 7.8 split by 2; 1 x 768 -> 768: 5.1, and 4.3 split by 4.)
+  // 1 x 1536 -> 12288, 96 CTAs unsplit: 7.5, and 8.6 split by 2; 1 x 768 -> 768:
+  // 5.1, and 4.3 split by 4.)
   int lg = 0;
   while (lg < 3 && (units << (lg + 1)) <= sms + sms / 8 && (2 << lg) <= kblocks &&
          ((8 << lg) <= kblocks || (units << (lg + 3)) <= sms))
@@ -815,24 +818,33 @@ static cudaError_t launch_few(const Fp8GemmArgs& a, int sms, cudaStream_t st) {
 
 cudaError_t fp8_gemm(const Fp8GemmArgs& a, int dev, cudaStream_t st) {
   const int sms = g_num_sms(dev);
-  // Few rows while one CTA per SM covers all tiles, in the smallest tile that
-  // does; beyond that the 128 x 256 tiles read less for each product.
-  auto fits = [&](int nt) { return fp8_blocks(a.out) * ((a.rows + nt - 1) / nt) <= sms; };
+  // Up to 32 rows the weights are read once either way, and the few-rows
+  // kernel is the faster one (16 x 4096 -> 9000: 8.5 us, and 20.7 in tiles of
+  // 128 rows; 32 x 768 -> 2304: 5.6 and 5.2).  Beyond, only where it can split
+  // a long sum over clusters (100 x 4096 -> 1536: 9.7 and 12.3; 64 x 4096 ->
+  // 4096: 10.0 and 12.2), not unsplit (65 x 4096 -> 4096: 13.8 and 12.3; 100 x
+  // 1536 -> 6144: 9.2 and 7.2) nor for a short one (64 x 768 -> 768: 5.7 and
+  // 5.3).
   if (a.rows <= 16) return launch_few<16>(a, sms, st);
-  if (a.rows <= 32 || fits(32)) return launch_few<32>(a, sms, st);
-  if (a.rows <= 64 || fits(64)) return launch_few<64>(a, sms, st);
+  if (a.rows <= 32 || (fp8_blocks(a.in) >= 8 && fp8_blocks(a.out) * ((a.rows + 31) / 32) * 2 <= sms + sms / 8))
+    return launch_few<32>(a, sms, st);
   CUtensorMap mx, my;
   if (!make_tmap_u8_pitch(&mx, a.x, a.rows, a.in, a.ldx, ManyCfg::BM)) return cudaErrorInvalidValue;
   if (!a.y_vec) my = mx;  // not used
   else if (!make_tmap_out(&my, a.y, a.rows, a.out, a.ldy, a.y_dtype == G4M_F32 ? 4 : 2, 32)) return cudaErrorInvalidValue;
   const long tiles = (a.rows + ManyCfg::BM - 1) / ManyCfg::BM * ((fp8_blocks(a.out) + 1) / 2);
   if (tiles > 0x3fffffffL) return cudaErrorInvalidValue;
+  // What does not fill the SMs once more is cut to use them all: narrower
+  // units are done and stored sooner (2304 x 768 -> 2304, 148 + 14 tiles: 14.9
+  // us whole, 12.9 in halves, 12.2 in quarters; 512 x 4096 -> 4096, 64 tiles:
+  // 18.2 whole, 14.6 in halves).
   const int rest = (int)(tiles % sms);
-  ManySplit cut;
-  cut.lg = 4 * rest <= sms ? 2 : 2 * rest <= sms ? 1 : 0;
-  cut.full = (int)tiles - (cut.lg ? rest : 0);
-  const int grid = tiles >= sms ? sms : (int)(tiles << cut.lg);
-  fp8_gemm_many_kernel<<<grid, ManyCfg::THREADS, ManyCfg::SMEM, st>>>(mx, my, a, cut);
+  const int lg = 4 * rest <= sms ? 2 : 2 * rest <= sms ? 1 : 0;
+  const int full = (int)tiles - rest, grid = tiles >= sms ? sms : rest << lg;
+  auto go = [&](auto kernel) { kernel<<<grid, ManyCfg::THREADS, ManyCfg::SMEM, st>>>(mx, my, a, full); };
+  if (rest == 0 || lg == 0) go(fp8_gemm_many_kernel<0>);
+  else if (lg == 1) go(fp8_gemm_many_kernel<1>);
+  else go(fp8_gemm_many_kernel<2>);
   return cudaGetLastError();
 }
 

@@ -242,6 +242,16 @@ def test_norm_options(ctx, native, opts, d):
     run_norm(ctx, native, **{**dict(rows=37, d=d, dtype="bf16", res="bf16", pad=0, off=0, rpg=5, outs="hnc", seed=d), **opts})
 
 
+@pytest.mark.parametrize("rows,d", [(9000, 1000), (9000, 1155), (4000, 4096), (700, 16384)])
+def test_rows_that_blocks_walk(ctx, native, rows, d):
+    """More rows than the grid holds at a time."""
+    run_norm(ctx, native, rows, d, "bf16", "f32", 0, 0, rpg=1000, outs="hnc", seed=d)
+    buf, x = rows_like(rows, 2 * d, 0, 0, torch.bfloat16, gen(d), 3.0)
+    c = Codes(rows, d)
+    ctx.fp8_quantize(x.data_ptr(), 1, 2 * d, rows, d, *c.args, act="silu", stream=stream())
+    assert_codes(c, *act64(x.double(), d, "silu"))
+
+
 @pytest.mark.parametrize("post", [True, False])
 @pytest.mark.parametrize("d", [256, 1024, 4096, 8192])
 def test_norm_one_sum_many_rows(ctx, native, post, d):
@@ -373,6 +383,19 @@ def test_linear(ctx, rows, i, o, dtype):
     bound = m * (4 * 33 * 2.0 ** -23 + (3 + (i + 127) // 128) * U) + H[dtype] * y.abs()
     bad = (got - y).abs() > bound
     assert not bad.any(), (bad.sum().item(), got[bad][:4], y[bad][:4], bound[bad][:4])
+
+
+@pytest.mark.parametrize("rows,i,o", [(33, 640, 40000), (70, 200, 9001), (90, 300, 37000), (150, 1300, 2561), (260, 100, 129), (390, 400, 9400),
+                                      (2500, 256, 2600), (3000, 200, 2049), (2400, 384, 2176), (5000, 128, 1000)])
+@pytest.mark.parametrize("dtype,pad,off", [("f32", 0, 0), ("f32", 1, 1), ("bf16", 8, 0), ("f16", 3, 1)])
+def test_linear_last_tiles(ctx, rows, i, o, dtype, pad, off):
+    """Numbers of 128 x 256 tiles below and above a multiple of the SMs, so
+    that the last ones are whole, halved or quartered.  Exact in f32; rounded
+    once otherwise."""
+    c, wc, sw, bias = linear_case(rows, i, o, rows + o, exact=True)
+    y = run_linear(ctx, c, wc, sw, bias, dtype, pad, off)
+    exp, _ = linear64(c, wc, sw, bias)
+    assert torch.equal(y, exp.to(DT[dtype][1]))
 
 
 def test_linear_nan_stays_in_its_row(ctx):
