@@ -17,13 +17,14 @@
 //              the order of arrival.
 //
 // What bounds them (B200, device time).  Many rows: 8192 x 4096 -> 8192 bf16
-// takes 252 us (2.18 PFLOP/s; 290 us and 1.9 PFLOP/s when repeated until the
+// takes 257 us (2.14 PFLOP/s; 290 us and 1.9 PFLOP/s when repeated until the
 // power cap holds the clock; a bf16 library product of that size would take
 // 332 us at its measured 1.65 PFLOP/s).  The MMAs of a block take 512 cycles;
 // its sums cross to the epilogue and back (issue 130, MMAs and their arrival
 // 600, loads and half of the sums 330, two wake-ups of about 200) in about
 // 1300 with two accumulators to hide them, and the f32 pipe is busy for 330.
-// TMEM holds no third accumulator of 256 columns.  Few rows: 1 x 4096 -> 32768
+// TMEM holds no third accumulator of 256 columns.  A call of
+// cut units alone takes about 4 us and 0.26 us for each column block.  Few rows: 1 x 4096 -> 32768
 // takes 25 us, 5.4 TB/s; below about 20 MB of weights a call is launch, set-up
 // (0.9 us), first bytes (0.8 us) and the cluster's exchange (0.7 us).
 //

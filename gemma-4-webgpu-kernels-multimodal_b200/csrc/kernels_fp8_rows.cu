@@ -159,7 +159,7 @@ __device__ __forceinline__ void scale8(float (&v)[8], float inv, const float* w,
 // place (rows off 16-byte boundaries) takes registers: those rows get more
 // threads with fewer chunks each, no loads ahead, and as many blocks as hide
 // each other's waits (2947 x 5193 bf16: 124 us with one block of 512 threads
-// an SM, 95 us with three of 384).
+// an SM, 95 us with three of 384; 76 since row edges are stored by a mask).
 template <int NCH, bool FULL>
 struct NormCfg {
   static constexpr int T = NCH == 4 ? 512 : FULL ? 256 : 384;
