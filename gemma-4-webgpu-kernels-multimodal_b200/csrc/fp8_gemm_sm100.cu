@@ -23,10 +23,10 @@
 // its sums cross to the epilogue and back (issue 130, MMAs and their arrival
 // 600, loads and half of the sums 330, two wake-ups of about 200) in about
 // 1300 with two accumulators to hide them, and the f32 pipe is busy for 330.
-// TMEM holds no third accumulator of 256 columns.  A call of
-// cut units alone takes about 4 us and 0.26 us for each column block.  Few rows: 1 x 4096 -> 32768
-// takes 25 us, 5.4 TB/s; below about 20 MB of weights a call is launch, set-up
-// (0.9 us), first bytes (0.8 us) and the cluster's exchange (0.7 us).
+// TMEM holds no third accumulator of 256 columns.  A call of cut units alone
+// takes about 4 us and 0.26 us for each column block.  Few rows: 1 x 4096 ->
+// 32768 takes 25 us, 5.4 TB/s; below about 20 MB of weights a call is launch,
+// set-up (0.9 us), first bytes (0.8 us) and the cluster's exchange (0.7 us).
 //
 // Every mbarrier wait is bounded; a timeout records an error word and the
 // CTA unwinds.
