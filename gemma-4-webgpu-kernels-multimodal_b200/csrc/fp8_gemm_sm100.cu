@@ -378,6 +378,11 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
     const float* scale = scales + half * C::BM + 32 * q + lane;
     uint32_t it = 0;
     bool ok = true, done = false, scaled = false;  // the next block's barriers, tested ahead
+    // Blocks of y sent so far, over all tiles: consecutive ones always take
+    // turns between the warp's two store blocks, so that all but the last
+    // store being read is enough before a block is written again, even after
+    // a tile that y's right edge left an odd number of blocks.
+    uint32_t sends = 0;
     // One of the share, COLS columns for this warp.
     auto complete = [&](int i, auto cols) {
       constexpr int COLS = decltype(cols)::value;
@@ -442,7 +447,6 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       // Rows of y that do not start on 16-byte boundaries leave by plain
       // stores, a warp's lanes side by side in a row.  (From the lane that
       // holds the row, 8192 x 4096 -> 8192 took three times as long.)
-      uint32_t sends = 0;
       auto send = [&](const uint4 (&o)[4], int col, int size) {
         uint8_t* block = stage + (sends++ & 1) * C::EPI_BLOCK;
         if (lane == 0) tma_store_read_wait<1>();

@@ -398,6 +398,26 @@ def test_linear_last_tiles(ctx, rows, i, o, dtype, pad, off):
     assert torch.equal(y, exp.to(DT[dtype][1]))
 
 
+@pytest.mark.parametrize("rows,i,o,dtype", [(128 * 700, 128, 1000, "f32"), (128 * 700, 128, 800, "bf16"), (128 * 300, 128, 2344, "f32"),
+                                            (128 * 460, 100, 40, "f32"), (128 * 460, 128, 24, "f16"), (128 * 75, 128, 1032, "f32")])
+def test_linear_odd_stores_then_more_tiles(ctx, rows, i, o, dtype):
+    """Tiles whose last store blocks number odd (y ends inside the tile), each
+    followed by further tiles of the same thread block with one column block
+    of sums: the store that still reads a block of shared memory and the next
+    tile's first write must not meet.  Exact sums, so any value of another
+    tile shows; repeated, as an overlap is a matter of time."""
+    c, wc, sw, bias = linear_case(rows, i, o, rows + o, exact=True, padded=False)
+    lin = ctx.fp8_linear(wc.view(torch.uint8).cpu().numpy(), sw.cpu().numpy(), bias.cpu().numpy())
+    y = torch.empty(rows, o, dtype=DT[dtype][1], device="cuda")
+    exp = linear64(c, wc, sw, bias)[0].to(DT[dtype][1])
+    for _ in range(8):
+        y.fill_(5.0)
+        for _ in range(3):
+            lin.run(*c.args, rows, y.data_ptr(), DT[dtype][0], o, stream=stream())
+        assert torch.equal(y, exp)
+    lin.close()
+
+
 def test_linear_nan_stays_in_its_row(ctx):
     """NaN codes, NaN and infinite scales reach only the rows (or the output blocks) they belong to."""
     for rows in (4, 200):
