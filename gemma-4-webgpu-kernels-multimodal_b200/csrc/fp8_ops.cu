@@ -103,10 +103,14 @@ int check_norm(const g4m_norm_args& a) {
   return rc;
 }
 
+// Device copy of n elements.  A copy from pageable memory may still be on its
+// way when cudaMemcpy returns, and no non-blocking stream waits for the legacy
+// stream that it runs on: it has landed before this returns.
 template <class T>
 bool to_device(T** dst, const T* src, size_t n) {
   return cudaMalloc(dst, n * sizeof(T)) == cudaSuccess &&
-         cudaMemcpy(*dst, src, n * sizeof(T), cudaMemcpyHostToDevice) == cudaSuccess;
+         cudaMemcpy(*dst, src, n * sizeof(T), cudaMemcpyHostToDevice) == cudaSuccess &&
+         cudaStreamSynchronize(cudaStreamLegacy) == cudaSuccess;
 }
 
 }  // namespace
@@ -313,6 +317,7 @@ int g4m_rope_prepare(g4m_ctx* ctx, int di, int head_dim, int rotary, const doubl
     R->interleaved = interleaved != 0;
     R->scale = (float)scale;
     if (!to_device(&R->turns, turns.data(), turns.size())) {
+      (void)cudaGetLastError();
       g4m_rope_free(R);
       return fail(G4M_E_CUDA, "rotary table upload failed");
     }

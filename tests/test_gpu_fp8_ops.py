@@ -540,6 +540,28 @@ def test_rope_far_and_negative_positions(ctx, native, dtype):
     rope.close()
 
 
+@pytest.mark.parametrize("hd", [64, 1024])
+def test_rope_runs_at_once_on_a_new_stream(ctx, native, hd):
+    """Prepared and run without a pause, on a stream that does not wait for
+    the legacy one, with the device busy there: the angles are complete."""
+    s = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+    pos = torch.arange(1, 6, device="cuda") * 1000
+    x = torch.randn(5, 2, hd, device="cuda", generator=gen(hd))
+    out = torch.empty_like(x)
+    for k in range(12):
+        f, _ = native.rope_frequencies(hd, 10000.0 + k)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            busy @ busy
+        rope = ctx.rope(hd, f)
+        rope.run(native.rope_view(x.data_ptr(), 2 * hd, hd, out.data_ptr(), 2 * hd, hd, 2), None, 0, 5, pos.data_ptr(), stream=s.cuda_stream)
+        torch.cuda.synchronize()
+        exp, mag = rope64(x, pos.cpu().numpy(), f, 1.0, False)
+        assert_rope(out, exp, mag, "f32", 5000)
+        rope.close()
+
+
 @pytest.mark.parametrize("hd,rotary", [(64, 64), (64, 48), (80, 20)])
 def test_rope_strides(ctx, native, hd, rotary):
     """Heads-major input (tokens inside heads), odd offsets and a broadcast head (stride 0) to separate outputs."""
