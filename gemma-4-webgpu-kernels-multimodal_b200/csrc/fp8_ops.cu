@@ -285,7 +285,8 @@ int g4m_rope_frequencies(int rotary, double theta, int scaling, double factor, d
       if (scaling == G4M_ROPE_YARN) keep = 1.0 - fmin(fmax((j - first) / fmax(last - first, 0.001), 0.0), 1.0);
       inv_freq[j] = scaling == G4M_ROPE_NONE ? f : keep * f + (1.0 - keep) * f / factor;
     }
-    *attention_scale = scaling == G4M_ROPE_YARN ? 0.1 * log(factor) + 1.0 : 1.0;
+    // only a stretch raises the attention's temperature
+    *attention_scale = scaling == G4M_ROPE_YARN && factor > 1.0 ? 0.1 * log(factor) + 1.0 : 1.0;
     return G4M_OK;
   });
 }

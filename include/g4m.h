@@ -215,7 +215,7 @@ enum g4m_rope_scaling {
   G4M_ROPE_NONE = 0,    /* theta^(-2 j / rotary) */
   G4M_ROPE_LINEAR = 1,  /* the same / factor */
   G4M_ROPE_BANDED = 2,  /* pairs with under `low` turns in `trained` positions / factor, over `high` kept, blended between */
-  G4M_ROPE_YARN = 3     /* the same split as a ramp over the pair index; attention scale 0.1 ln(factor) + 1 */
+  G4M_ROPE_YARN = 3     /* the same split as a ramp over the pair index; attention scale 0.1 ln(max(factor, 1)) + 1 */
 };
 /* Host helper: fills inv_freq[rotary / 2] and *attention_scale. */
 G4M_API int g4m_rope_frequencies(int rotary, double theta, int scaling, double factor, double low, double high,

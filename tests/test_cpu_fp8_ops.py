@@ -103,6 +103,14 @@ def test_rope_frequencies(native, rotary, theta):
     assert abs(m - (0.1 * np.log(16) + 1)) < 1e-15
 
 
+@pytest.mark.parametrize("factor,scale", [(0.25, 1.0), (0.999, 1.0), (1.0, 1.0), (1.5, 0.1 * np.log(1.5) + 1), (40.0, 0.1 * np.log(40.0) + 1)])
+def test_rope_yarn_scale_never_shrinks(native, factor, scale):
+    """Factors up to 1 leave the attention scale at 1; the frequencies follow the factor either way."""
+    f, m = native.rope_frequencies(64, 10000.0, "yarn", factor=factor, low=1.0, high=32.0, trained=4096)
+    assert abs(m - scale) < 1e-15
+    np.testing.assert_allclose(f[-1], 10000.0 ** (-62 / 64) / factor, rtol=2.0 ** -48)
+
+
 def test_python_side_refuses(native):
     """Shapes that the bindings know are refused before anything reaches the library."""
     class Ctx:
