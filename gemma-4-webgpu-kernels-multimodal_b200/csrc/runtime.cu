@@ -1117,8 +1117,10 @@ int g4m_profile_begin(g4m_ctx* ctx, int di) {
   if (!ctx || di < 0 || di >= (int)ctx->devs.size()) return fail(G4M_E_ARG, "bad context or device index");
   Device& d = *ctx->devs[di];
   std::lock_guard<std::mutex> lk(d.mu);
+  std::lock_guard<std::mutex> lp(d.prof_mu);
+  for (const ProfRec& r : d.prof) d.give_back(r);
   d.prof.clear();
-  d.ev_used = 0;
+  ++d.prof_session;
   d.prof_on = true;
   return G4M_OK;
 }
@@ -1128,12 +1130,19 @@ int g4m_profile_end(g4m_ctx* ctx, int di, char* buf, size_t cap) {
   Device& d = *ctx->devs[di];
   std::lock_guard<std::mutex> lk(d.mu);
   cudaSetDevice(d.id);
-  d.prof_on = false;
+  std::vector<ProfRec> recs;
+  {
+    std::lock_guard<std::mutex> lp(d.prof_mu);
+    d.prof_on = false;
+    recs.swap(d.prof);
+  }
   std::vector<std::string> labels;
   std::vector<double> ms;
   std::vector<long> cnt;
-  for (const ProfRec& r : d.prof) {
-    if (cudaEventSynchronize(r.b) != cudaSuccess) return fail(G4M_E_CUDA, "profile event wait failed");
+  cudaError_t waited = cudaSuccess;
+  for (const ProfRec& r : recs) {
+    if (waited == cudaSuccess) waited = cudaEventSynchronize(r.b);
+    if (waited != cudaSuccess) break;
     float t = 0.f;
     cudaEventElapsedTime(&t, r.a, r.b);
     size_t i = 0;
@@ -1146,6 +1155,11 @@ int g4m_profile_end(g4m_ctx* ctx, int di, char* buf, size_t cap) {
     ms[i] += t;
     cnt[i] += 1;
   }
+  {
+    std::lock_guard<std::mutex> lp(d.prof_mu);
+    for (const ProfRec& r : recs) d.give_back(r);
+  }
+  if (waited != cudaSuccess) return fail(G4M_E_CUDA, "profile event wait failed");
   std::string js = "{";
   for (size_t i = 0; i < labels.size(); ++i) {
     char tmp[160];
@@ -1153,8 +1167,6 @@ int g4m_profile_end(g4m_ctx* ctx, int di, char* buf, size_t cap) {
     js += tmp;
   }
   js += "}";
-  d.prof.clear();
-  d.ev_used = 0;
   if (js.size() + 1 > cap) return fail(G4M_E_ARG, "profile buffer too small");
   memcpy(buf, js.c_str(), js.size() + 1);
   return G4M_OK;

@@ -118,20 +118,24 @@ inline int quant_group(const float* s, int n) {
   return nz == 0 ? 0 : (nz == n ? 1 : -1);
 }
 
-// Opt-in per-launch event timing (g4m_profile_begin / g4m_profile_end).
+// Opt-in per-launch event timing (g4m_profile_begin / g4m_profile_end).  A
+// launch keeps its record to itself until both events are recorded; what the
+// device holds of it is behind prof_mu, as calls need not hold Device::mu.
 struct ProfRec {
-  const char* label;
-  cudaEvent_t a, b;
+  const char* label = nullptr;
+  cudaEvent_t a = nullptr, b = nullptr;  // null: not timed
+  unsigned session = 0;                  // of the g4m_profile_begin that it belongs to
 };
 
 extern std::atomic<long long> g_launches;
 
 struct Device {
   int id = 0;
-  bool prof_on = false;
+  std::atomic<bool> prof_on{false};
+  std::mutex prof_mu;  // taken after mu where both are held
+  unsigned prof_session = 0;
   std::vector<ProfRec> prof;
-  std::vector<cudaEvent_t> ev_pool;
-  size_t ev_used = 0;
+  std::vector<cudaEvent_t> ev_free;
   cudaStream_t st = nullptr;   // compute
   cudaStream_t cst = nullptr;  // host <-> device copies of the batch calls (overlap the compute of other chunks)
   int* err = nullptr;
@@ -149,18 +153,27 @@ struct Device {
   int aw_mel_sr = 0;  // sampling rate the mel filter bank was built for
   std::mutex mu;
 
-  cudaEvent_t next_event() {
-    if (ev_used == ev_pool.size()) {
-      cudaEvent_t e;
-      cudaEventCreate(&e);
-      ev_pool.push_back(e);
+  // With prof_mu held; null when no event can be made.
+  cudaEvent_t take_event() {
+    cudaEvent_t e = nullptr;
+    if (!ev_free.empty()) {
+      e = ev_free.back();
+      ev_free.pop_back();
+    } else if (cudaEventCreate(&e) != cudaSuccess) {
+      e = nullptr;
     }
-    return ev_pool[ev_used++];
+    return e;
+  }
+  void give_back(const ProfRec& r) {
+    for (cudaEvent_t e : {r.a, r.b})
+      if (e) ev_free.push_back(e);
   }
 
   void free_all() {
-    for (cudaEvent_t e : ev_pool) cudaEventDestroy(e);
-    ev_pool.clear();
+    for (const ProfRec& r : prof) give_back(r);
+    prof.clear();
+    for (cudaEvent_t e : ev_free) cudaEventDestroy(e);
+    ev_free.clear();
     for (void* p : allocs) cudaFree(p);
     allocs.clear();
     DevBuf* bufs[] = {&vb.h, &vb.y, &vb.h0, &vb.a_hi, &vb.a_lo, &vb.a_c, &vb.o_hi, &vb.o_lo, &vb.g_hi, &vb.g_lo,
@@ -216,24 +229,43 @@ inline std::vector<std::pair<int, int>> edge_chunks(int n, int edge, int mid) {
   return c;
 }
 
-inline void prof_begin(Device& d, cudaStream_t st, const char* label) {
+inline ProfRec prof_begin(Device& d, cudaStream_t st, const char* label) {
   g_launches.fetch_add(1, std::memory_order_relaxed);
-  if (!d.prof_on) return;
-  ProfRec r{label, d.next_event(), d.next_event()};
+  ProfRec r;
+  if (!d.prof_on.load(std::memory_order_relaxed)) return r;
+  // An event recorded into a graph has no time that could be asked for.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+    (void)cudaGetLastError();
+    return r;
+  }
+  {
+    std::lock_guard<std::mutex> lk(d.prof_mu);
+    if (!d.prof_on.load(std::memory_order_relaxed)) return r;
+    r = {label, d.take_event(), d.take_event(), d.prof_session};
+    if (!r.a || !r.b) {
+      d.give_back(r);
+      return ProfRec();
+    }
+  }
   cudaEventRecord(r.a, st);
-  d.prof.push_back(r);
+  return r;
 }
-inline void prof_end(Device& d, cudaStream_t st) {
-  if (d.prof_on && !d.prof.empty()) cudaEventRecord(d.prof.back().b, st);
+inline void prof_end(Device& d, cudaStream_t st, const ProfRec& r) {
+  if (!r.a) return;
+  cudaEventRecord(r.b, st);
+  std::lock_guard<std::mutex> lk(d.prof_mu);
+  if (d.prof_on.load(std::memory_order_relaxed) && r.session == d.prof_session) d.prof.push_back(r);
+  else d.give_back(r);
 }
 
 // Launch a kernel through a launcher returning cudaError_t, counting it and,
 // when profiling is on, bracketing it with events under `label`.
 #define G4M_RUN(label, x)                                                                            \
   do {                                                                                               \
-    ::g4m::prof_begin(d, st, label);                                                                 \
+    const ::g4m::ProfRec prof_ = ::g4m::prof_begin(d, st, label);                                    \
     cudaError_t e_ = (x);                                                                            \
-    ::g4m::prof_end(d, st);                                                                          \
+    ::g4m::prof_end(d, st, prof_);                                                                   \
     if (e_ != cudaSuccess) return ::g4m::fail(G4M_E_CUDA, std::string(label) + ": " + cudaGetErrorString(e_)); \
   } while (0)
 void* dalloc(Device& d, size_t bytes);

@@ -344,7 +344,8 @@ G4M_API int g4m_selftest_wait_timeout(g4m_ctx* ctx, int device_index, long long 
 
 /* Per-launch CUDA-event timing on one device: begin, run calls, end.  The
  * end call waits for the recorded events and writes a JSON object
- * {"label": [launches, total_ms], ...} into buf. */
+ * {"label": [launches, total_ms], ...} into buf.  Calls of any thread are
+ * counted that return between the two; launches captured into a graph are not. */
 G4M_API int g4m_profile_begin(g4m_ctx* ctx, int device_index);
 G4M_API int g4m_profile_end(g4m_ctx* ctx, int device_index, char* buf, size_t cap);
 

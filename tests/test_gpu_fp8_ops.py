@@ -829,6 +829,68 @@ def test_two_host_threads(ctx, native):
     assert not failed, failed
 
 
+PER_LAYER = {"norm_residual": 3, "fp8_gemm": 3, "rope": 1, "fp8_quantize": 1}
+
+
+def test_profile_leaves_captures_alone(ctx, native):
+    """With per-launch timing on, a capture still works, and only the eager
+    launches are timed."""
+    layer = Layer(ctx, native, 5, 8)
+    layer.run()
+    torch.cuda.synchronize()
+    ctx.profile_begin()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        layer.run()
+    for _ in range(2):
+        layer.run()
+    g.replay()
+    got = ctx.profile_end()
+    assert {k: v[0] for k, v in got.items()} == {k: 2 * n for k, n in PER_LAYER.items()}
+    assert all(0 < v[1] < 1e3 for v in got.values())
+    torch.cuda.synchronize()
+    layer.check()
+    ctx.profile_begin()
+    assert ctx.profile_end() == {}
+
+
+def test_profile_counts_every_thread(ctx, native):
+    """Launches of several threads are timed at once; timing that another
+    thread ends and begins meanwhile loses some and breaks nothing."""
+    import threading
+    layers = [Layer(ctx, native, 3, 10 + k) for k in range(4)]
+    for layer in layers:
+        layer.run()
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(layer):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    layer.run()
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # a thread's exception would be lost
+            failed.append(repr(e))
+
+    for switch in (False, True):
+        ctx.profile_begin()
+        threads = [threading.Thread(target=work, args=(layer,)) for layer in layers]
+        for t in threads:
+            t.start()
+        while switch and any(t.is_alive() for t in threads):
+            ctx.profile_end()
+            ctx.profile_begin()
+        for t in threads:
+            t.join()
+        got = {k: v[0] for k, v in ctx.profile_end().items()}
+        assert not failed, failed
+        if not switch:
+            assert got == {k: 4 * 60 * n for k, n in PER_LAYER.items()}
+    for layer in layers:
+        layer.check()
+
+
 def test_default_stream_is_the_legacy_one(ctx):
     """Stream 0 orders with torch's default stream."""
     x = torch.zeros(64, 4096, device="cuda")
