@@ -42,6 +42,7 @@ _SIGS = [
     ("g4m_vision_embed_images", _I, [_VP, _I, _VP, _VP, _VP, _I, _I, _I, _VP, _VP, _VP]),
     ("g4m_resize_rgb", _I, [_VP, _I, _VP, _I, _I, _I, _I, _I, _VP]),
     ("g4m_selftest_wait_timeout", _I, [_VP, _I, ctypes.c_longlong]),
+    ("g4m_synchronize", _I, [_VP, _I, _VP]),
     ("g4m_fp8_quantize", _I, [_VP, _I, _I, _VP, _I, _I64, _I64, _I, _VP, _VP]),
     ("g4m_fp8_linear_prepare", _I, [_VP, _I, _VP, _VP, _I, _I, _VP, ctypes.POINTER(_VP)]),
     ("g4m_fp8_linear_run", _I, [_VP, _VP, _I64, _VP, _I, _I64, _VP]),
@@ -324,6 +325,11 @@ class Context:
                                            ptr(lengths), sampling_rate, layer_count, int(max_samples),
                                            ctypes.c_void_p(out_ptr), ptr(rows), ctypes.c_void_p(stream) if stream else None))
         return rows
+
+    def synchronize(self, stream: int = 0, device=0) -> None:
+        """Wait for the stream; raises E_TIMEOUT when a device-side wait expired
+        in a call since the last report."""
+        check(lib().g4m_synchronize(self.h, device, stream or None))
 
     def fp8_quantize(self, x: int, dtype: int, ldx: int, rows: int, d: int, codes: int, ldc: int, scales: int, lds: int,
                      act="none", stream: int = 0, device=0) -> None:

@@ -283,9 +283,6 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
         const int bytes = two ? kFp8TileBytes : WIDTH * 128;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % C::STAGES;
-          // An earlier kernel on this device failed: looked up once the first
-          // copies are on their way.
-          if (it == C::STAGES && *reinterpret_cast<volatile int*>(a.err) != 0) abort_flag = 1;
           if (!mbar_wait(&bar_done[s], ((it / C::STAGES) & 1) ^ 1, a.err, kErrWaitEmpty, &abort_flag)) {
             ok = false;
             break;
@@ -601,9 +598,6 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
       int it = 0;
       for (; it < nk; ++it) {
         const int s = it % C::STAGES;
-        // An earlier kernel on this device failed: looked up once the first
-        // copies are on their way.
-        if (it == C::STAGES && *reinterpret_cast<volatile int*>(a.err) != 0) abort_flag = 1;
         if (!mbar_wait(&bar_done[s], ((it / C::STAGES) & 1) ^ 1, a.err, kErrWaitEmpty, &abort_flag)) break;
         uint8_t* sw = smem + s * C::STAGE_BYTES;
         mbar_expect_tx(&bar_full[s], C::STAGE_BYTES);

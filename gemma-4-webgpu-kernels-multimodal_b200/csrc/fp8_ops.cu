@@ -117,6 +117,15 @@ bool to_device(T** dst, const T* src, size_t n) {
 
 extern "C" {
 
+int g4m_synchronize(g4m_ctx* ctx, int di, void* stream) {
+  return no_throw([&]() -> int {
+    if (!device_ok(ctx, di)) return fail(G4M_E_ARG, "bad context or device index");
+    Device& d = *ctx->devs[di];
+    DeviceGuard guard(d.id);
+    return finish(d, stream_of(stream));
+  });
+}
+
 int g4m_fp8_quantize(g4m_ctx* ctx, int di, int act, const void* x, int dtype, int64_t ldx, int64_t rows, int cols,
                      const g4m_fp8_rows* out, void* stream) {
   return no_throw([&]() -> int {

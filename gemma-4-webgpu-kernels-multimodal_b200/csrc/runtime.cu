@@ -56,6 +56,7 @@ int finish(Device& d, cudaStream_t st) {
   if (e != cudaSuccess) return fail(G4M_E_CUDA, std::string("error word read: ") + cudaGetErrorString(e));
   if (w != 0) {
     cudaMemset(d.err, 0, sizeof(int));
+    cudaStreamSynchronize(cudaStreamLegacy);  // cleared before any later launch, on whichever stream
     return fail(G4M_E_TIMEOUT, "a device-side bounded wait expired (kernel error code " + std::to_string(w) + ")");
   }
   return G4M_OK;
@@ -1052,14 +1053,16 @@ int g4m_vision_embed_images(g4m_ctx* ctx, int n, const uint8_t* const* images, c
 }
 
 int g4m_selftest_wait_timeout(g4m_ctx* ctx, int di, long long budget_cycles) {
-  if (!ctx || di < 0 || di >= (int)ctx->devs.size() || budget_cycles <= 0 || budget_cycles > 4000000000LL)
+  if (!ctx || di < 0 || di >= (int)ctx->devs.size() || budget_cycles == 0 || budget_cycles > 4000000000LL ||
+      budget_cycles < -4000000000LL)
     return fail(G4M_E_ARG, "bad argument");
   Device& d = *ctx->devs[di];
   std::lock_guard<std::mutex> lk(d.mu);
   cudaSetDevice(d.id);
   (void)cudaGetLastError();
   cudaStream_t st = d.st;
-  G4M_RUN("selftest_wait", selftest_wait_timeout(d.err, budget_cycles, st));
+  G4M_RUN("selftest_wait", selftest_wait_timeout(d.err, budget_cycles < 0 ? -budget_cycles : budget_cycles, st));
+  if (budget_cycles < 0) return G4M_OK;
   return finish(d, st);  // reads and clears the error word: G4M_E_TIMEOUT expected
 }
 

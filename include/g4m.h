@@ -125,9 +125,17 @@ G4M_API int g4m_linear_run_noalloc(g4m_linear* lin, const float* x_dev, int rows
  * (G4M_E_ARG otherwise), 16-byte aligned rows are faster.  Zero rows are
  * G4M_OK and launch nothing.  Nothing outside the stated rows and columns is
  * read or written.  Inputs and outputs must not overlap except where stated.
- * All are inference operators: none has a backward form.  A device-side wait
- * that expires shows as G4M_E_TIMEOUT in the next call that waits for the
- * device (as with g4m_linear_run). */
+ * All are inference operators: none has a backward form.  None of them waits
+ * for the device, so none reports a device-side wait that expired in an
+ * earlier call: g4m_synchronize does. */
+
+/* Wait for `stream` (NULL = the device's legacy default stream; not one that
+ * is being captured).  G4M_E_TIMEOUT when a bounded wait of any kernel on the
+ * device has expired since the last call that reported one: the outputs of
+ * calls made since then are not to be trusted.  The error is cleared and the
+ * context stays usable.  Calls on host memory (g4m_qat_linear, the embed
+ * calls) wait themselves and report the same way. */
+G4M_API int g4m_synchronize(g4m_ctx* ctx, int device_index, void* stream);
 
 enum g4m_dtype { G4M_F32 = 0, G4M_BF16 = 1, G4M_F16 = 2 };
 
@@ -339,7 +347,8 @@ G4M_API double g4m_checksum_floats(const float* values, int64_t count);
  * kernels' bounded wait with a budget of budget_cycles (1 .. 4e9), and
  * returns the resulting status: G4M_E_TIMEOUT with the kernel's error code in
  * g4m_last_error().  The error word is cleared, so the context stays usable.
- * Nothing faults or hangs. */
+ * Nothing faults or hangs.  A negative budget launches the same wait and
+ * returns G4M_OK without waiting for it: the next call that waits reports it. */
 G4M_API int g4m_selftest_wait_timeout(g4m_ctx* ctx, int device_index, long long budget_cycles);
 
 /* Per-launch CUDA-event timing on one device: begin, run calls, end.  The

@@ -65,6 +65,11 @@ def test_handles_refuse(native):
     L.g4m_rope_free(None)
 
 
+def test_synchronize_refuses(native):
+    assert native.lib().g4m_synchronize(None, 0, None) == ARG and "context" in native.last_error()
+    assert native.lib().g4m_selftest_wait_timeout(None, 0, -5) == ARG
+
+
 @pytest.mark.parametrize("bad,status", [
     (dict(rotary=7), SHAPE), (dict(rotary=0), SHAPE), (dict(theta=0.0), ARG), (dict(theta=float("nan")), ARG),
     (dict(scaling="linear", factor=0.0), ARG), (dict(scaling="banded", factor=2.0, low=4.0, high=4.0, trained=64), ARG),

@@ -829,6 +829,24 @@ def test_two_host_threads(ctx, native):
     assert not failed, failed
 
 
+@pytest.mark.parametrize("rows", [3, 700])
+def test_an_expired_wait_is_reported(ctx, native, rows):
+    """A wait that ran out in an earlier call: the linear's own sums stand all
+    the same, and the next call that waits says so, once."""
+    c, wc, sw, bias = linear_case(rows, 2048, 300, 4, exact=True)
+    exp = linear64(c, wc, sw, bias)[0]
+    ctx.synchronize(stream())
+    assert native.lib().g4m_selftest_wait_timeout(ctx.h, 0, -200_000) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(run_linear(ctx, c, wc, sw, bias, "f32").double(), exp)
+    with pytest.raises(native.G4MError) as e:
+        ctx.synchronize(stream())
+    assert e.value.status == 5 and "kernel error code 1" in str(e.value)
+    ctx.synchronize(stream())
+    assert torch.equal(run_linear(ctx, c, wc, sw, bias, "f32").double(), exp)
+    ctx.synchronize()
+
+
 PER_LAYER = {"norm_residual": 3, "fp8_gemm": 3, "rope": 1, "fp8_quantize": 1}
 
 
