@@ -168,7 +168,9 @@ __device__ __forceinline__ void cluster_push(uint32_t remote, const void* src, u
                : "memory");
 }
 
-// The producer's waits for copies that nobody has consumed after a timeout.
+// Waits for what is still on its way after a timeout: copies that nobody has
+// consumed, MMAs whose sums nobody takes, totals from the cluster.  A CTA that
+// left before would let them write memory that is no longer its own.
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, int* err) {
   const uint32_t b = smem_u32(bar);
   const long long t0 = clock64();
@@ -299,8 +301,7 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
     }
     if (warp == 1) {
       // bar_done of a stage tells both that the stage is free and that the
-      // block's sums are complete; the epilogue waits for every one, so no
-      // arrival is on its way when the CTA exits.
+      // block's sums are complete.
       const uint64_t dbase = desc_k_sw128(smem_u32(smem));
       uint32_t it = 0;
       bool full = false, free = true;  // tested ahead
@@ -321,6 +322,8 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       };
       const bool ok = issue((long)whole * kblocks, idesc_e4m3_f32(C::BM, C::BN));
       if (unit && ok) issue((long)share * kblocks, idesc_e4m3_f32(C::BM, WIDTH));
+      // Whatever became of the epilogue, the CTA outlives its MMAs.
+      if (lane == 0 && it > 0) drain(&bar_done[(it - 1) % C::STAGES], ((it - 1) / C::STAGES) & 1, a.err);
     }
     if (warp >= 2) {
       // Scale products of one output block (half of the tile): slot it % 2
@@ -609,7 +612,8 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
   } else if (warp == 1) {
     constexpr uint32_t idesc = idesc_e4m3_f32(128, NT);
     const uint64_t dbase = desc_k_sw128(smem_u32(smem));
-    for (int it = 0; it < nk; ++it) {
+    int it = 0;
+    for (; it < nk; ++it) {
       const int s = it % C::STAGES;
       const uint32_t turn = (it / C::STAGES) & 1;
       const uint64_t dw = desc_add(dbase, s * C::STAGE_BYTES);
@@ -619,6 +623,8 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
       tc_fence_after();
       mma_block(tmem_base + s * NT, dw, desc_add(dw, C::W_BYTES), idesc, &bar_done[s]);
     }
+    // Whatever became of the epilogue, the CTA outlives its MMAs.
+    if (lane == 0 && it > 0) drain(&bar_done[(it - 1) % C::STAGES], ((it - 1) / C::STAGES) & 1, a.err);
   } else {
     const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16);
     const float* swp = a.sw + (long)ob * kblocks + k0;
@@ -716,6 +722,7 @@ __global__ void __launch_bounds__(FewCfg<NT>::THREADS, 2)
       }
       __syncwarp();
       ok = warp_wait(bar_part, 0, a.err, kErrWaitAccFull, &abort_flag);
+      if (!ok && lane == 0) drain(bar_part, 0, a.err);
       if (ok && o < a.out)
         with_type(a.y_dtype, [&](auto* tp) {
           auto* y = static_cast<decltype(tp)>(a.y) + (row0 + j0) * a.ldy + o;
