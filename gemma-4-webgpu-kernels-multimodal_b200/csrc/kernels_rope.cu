@@ -3,8 +3,8 @@
 //
 // The angle of (token, pair) is position * frequency modulo one turn.  The
 // frequency is kept as a 64-bit fixed-point fraction of a turn, so the
-// integer product wraps modulo one turn by itself and the phase is exact to
-// position * 2^-65 turns at any position, without a 64-bit float operation.
+// integer product wraps modulo one turn by itself and the phase is off by at
+// most |position| * 2^-65 turns, without a 64-bit float operation.
 // A block computes the cosines and sines of its tokens once into shared
 // memory; a thread then keeps those of its pairs in registers and walks the
 // heads, the next one's loads in flight.  A warp covers one token's
@@ -71,9 +71,14 @@ __device__ __forceinline__ void rope_table(const RopeArgs& a, float2* cs, long t
     const int t = i / a.half, j = i - t * a.half;
     const long pos = a.pos64 ? static_cast<const long*>(a.positions)[t0 + t] : static_cast<const int*>(a.positions)[t0 + t];
     const uint64_t phase = (uint64_t)pos * a.turns[j];
+    // The nearest quarter turn comes off in integers, so that the rounding to
+    // f32 is relative to what is left, at most an eighth of a turn.
+    const uint64_t quarter = (phase + (1ull << 61)) >> 62;
+    const long long rest = (long long)(phase - (quarter << 62));
     float sn, cn;
-    sincospif(__ll2float_rn((long long)phase) * 0x1p-63f, &sn, &cn);  // half turns in [-1, 1]
-    cs[i] = make_float2(cn * a.scale, sn * a.scale);
+    sincospif(__ll2float_rn(rest) * 0x1p-63f, &sn, &cn);  // half turns in [-1/4, 1/4]
+    const float c = quarter & 1 ? sn : cn, s = quarter & 1 ? cn : sn;
+    cs[i] = make_float2((quarter + 1) & 2 ? -c * a.scale : c * a.scale, quarter & 2 ? -s * a.scale : s * a.scale);
   }
 }
 

@@ -562,6 +562,32 @@ def test_rope_runs_at_once_on_a_new_stream(ctx, native, hd):
         rope.close()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_cosines_and_sines(ctx, native, interleaved):
+    """Pairs (1, 0) come back as (cos, sin), each with a relative error: the
+    phase less its nearest quarter turn rounded to f32 (2^-24 of an angle of at
+    most pi/4: no more of its sine or cosine), and the function's unit in the
+    last place (2^-23).  Absolute, what position and frequency leave in the
+    phase: 2^20 positions * 2^-61 turns * 2 pi."""
+    tokens, r = 4000, 128
+    g = gen(31)
+    pos = torch.randint(-(1 << 20), 1 << 20, (tokens,), device="cuda", generator=g)
+    f, _ = native.rope_frequencies(r, 10000.0)
+    # quarter turns, halves and what lies next to them
+    f[:8] = 2 * math.pi * np.array([0.25, 0.5, 0.75, 0.125, 0.25 + 2.0 ** -40, 0.5 - 2.0 ** -40, 0.375, 2.0 ** -30])
+    x = torch.zeros(tokens, r, device="cuda")
+    x[:, 0::2 if interleaved else 1][:, :r // 2] = 1.0
+    rope = ctx.rope(r, f, interleaved)
+    out = torch.empty_like(x)
+    rope.run(native.rope_view(x.data_ptr(), r, r, out.data_ptr(), r, r, 1), None, 0, tokens, pos.data_ptr(), stream=stream())
+    cos, sin = rope_angles(pos.cpu().numpy(), f)
+    got = (out[:, 0::2], out[:, 1::2]) if interleaved else (out[:, :r // 2], out[:, r // 2:])
+    for v, exp in zip(got, (cos, sin)):
+        bad = (v.double() - exp).abs() > exp.abs() * 3 * U + 2.0 ** 20 * 2.0 ** -61 * 2 * math.pi
+        assert not bad.any(), (bad.sum().item(), v[bad][:4], exp[bad][:4])
+    rope.close()
+
+
 @pytest.mark.parametrize("hd,rotary", [(64, 64), (64, 48), (80, 20)])
 def test_rope_strides(ctx, native, hd, rotary):
     """Heads-major input (tokens inside heads), odd offsets and a broadcast head (stride 0) to separate outputs."""
