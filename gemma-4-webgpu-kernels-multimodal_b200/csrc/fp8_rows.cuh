@@ -290,18 +290,20 @@ __device__ __forceinline__ uint2 fp8_encode8(const float (&v)[8], float s) {
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
   inv = fmaf(fmaf(-s, inv, 1.0f), inv, inv);  // one Newton step
-  const uint64_t inv2 = pack_f32x2(inv, inv), neg2 = pack_f32x2(-s, -s);
+  const uint64_t s2 = pack_f32x2(s, s), neg2 = pack_f32x2(-inv, -inv);
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // div_by_rcp of two
-    const uint64_t x = pack_f32x2(v[2 * i], v[2 * i + 1]), q = mul_f32x2(x, inv2);
+  for (int i = 0; i < 4; ++i) {
+    // div_by_rcp of two, with the sign turned until the code: so a zero keeps
+    // its own (a residual of +0 added to a quotient of -0 would make it +0).
+    const uint64_t x = pack_f32x2(v[2 * i], v[2 * i + 1]), q = mul_f32x2(x, neg2);
     float q0, q1;
-    unpack_f32x2(fma3_f32x2(fma3_f32x2(q, neg2, x), inv2, q), q0, q1);
+    unpack_f32x2(fma3_f32x2(fma3_f32x2(q, s2, x), neg2, q), q0, q1);
     uint16_t p;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p) : "f"(q1), "f"(q0));
     w[i] = p;
   }
-  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+  return make_uint2((w[0] | (w[1] << 16)) ^ 0x80808080u, (w[2] | (w[3] << 16)) ^ 0x80808080u);
 }
 
 // Codes [c, c + 8) of a row of d codes that starts on a 16-byte boundary.

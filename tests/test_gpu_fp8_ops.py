@@ -124,6 +124,31 @@ def test_quantize(ctx, rows, d, pad, off, dtype, act):
         assert torch.equal(c.codes().view(torch.uint8), q.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_quantize_keeps_the_sign_of_zero(ctx, native, dtype):
+    """Codes of zeros and of values that round to zero carry their sign, as a
+    true division's do: from the quantiser and from the norm."""
+    g = gen(77)
+    x = torch.randn(40, 384, device="cuda", generator=g)
+    x *= torch.randint(0, 2, x.shape, device="cuda", generator=g)  # zeros of either sign
+    x[3] = 0.0
+    x[4] = -0.0
+    x[5, 1:] *= 2.0 ** -12
+    x = x.to(DT[dtype][1])
+    assert (x.double().signbit() & (x == 0)).any()
+    s = torch.from_numpy(block_amax(x.float()).clamp_min(FLOOR).cpu().numpy() / np.float32(448)).cuda()
+    exp = (x.float() / s.repeat_interleave(128, 1)).to(torch.float8_e4m3fn).view(torch.uint8)
+    c, n = Codes(40, 384), Codes(40, 384)
+    ctx.fp8_quantize(x.data_ptr(), DT[dtype][0], 384, 40, 384, *c.args, stream=stream())
+    ctx.norm_residual(native.norm_args(rows=40, d=384, dtype=DT[dtype][0], h_dtype=DT[dtype][0], eps=0.0, h=x.data_ptr(), ldh=384, **n.fields),
+                      stream=stream())
+    assert torch.equal(c.scales(), s.t()) and torch.equal(n.scales(), s.t())
+    assert torch.equal(c.codes().view(torch.uint8), exp)
+    # the norm adds its absent branch: h + 1 * (+0), which makes -0 a +0
+    zero = x == 0
+    assert torch.equal(n.codes().view(torch.uint8)[~zero], exp[~zero]) and (n.codes().view(torch.uint8)[zero] == 0).all()
+
+
 def test_quantize_special_blocks(ctx):
     """Zeros, the least and largest magnitudes, and blocks with an infinity or NaN: those read NaN whole, their neighbours are not touched by it."""
     x = torch.ones(8, 300, device="cuda")
