@@ -124,6 +124,35 @@ def test_quantize(ctx, rows, d, pad, off, dtype, act):
         assert torch.equal(c.codes().view(torch.uint8), q.view(torch.uint8))
 
 
+def test_quantize_next_to_ties(ctx):
+    """Quotients within a few units of the borders between codes, for scales of
+    all kinds, the all-ones mantissa among them: bit for bit those of a true
+    division."""
+    rng = np.random.default_rng(5)
+    v = np.arange(127, dtype=np.uint8)  # the magnitudes, and the borders between them
+    mag = torch.from_numpy(v).view(torch.float8_e4m3fn).double().numpy()
+    ties = (mag[1:] + mag[:-1]) / 2
+    amax = [np.float32((3.5 - 2.0 ** -22) * 2.0 ** k) for k in range(-90, 120, 3)]
+    amax += [np.float32(m * 2.0 ** k) for m, k in zip(rng.uniform(1, 2, 3000), rng.integers(-94, 126, 3000))]
+    x = np.zeros((len(amax), 256), np.float32)
+    for r, a in enumerate(amax):
+        s = np.float32(a) / np.float32(448)
+        near = (ties * np.float64(s)).astype(np.float32)
+        x[r, :126], x[r, 128:254] = near, -near
+        step = rng.integers(-2, 3, 256).astype(np.int32)
+        x[r] = np.where(x[r] != 0, (x[r].view(np.int32) + step).view(np.float32), 0)
+        x[r, 126:128], x[r, 254:] = (a, np.float32(2.0 ** -17) * a / np.float32(3.5)), (-a, -a * np.float32(2.0 ** -19))
+    x = np.where(np.abs(x) > np.array(amax, np.float32)[:, None], np.array(amax, np.float32)[:, None], x)
+    x[:70, 127], x[:70, 255] = [2.0 ** (k - 17) for k in range(-90, 120, 3)], [-(2.0 ** (k - 17)) for k in range(-90, 120, 3)]
+    s = (np.array(amax, np.float32) / np.float32(448))[:, None]
+    exp = torch.from_numpy(x / s).to(torch.float8_e4m3fn).view(torch.uint8)
+    c, xd = Codes(len(amax), 256), torch.from_numpy(x).cuda()
+    ctx.fp8_quantize(xd.data_ptr(), 0, 256, len(amax), 256, *c.args, stream=stream())
+    assert torch.equal(c.scales().cpu(), torch.from_numpy(np.repeat(s.T, 2, 0)))
+    bad = c.codes().view(torch.uint8).cpu() != exp
+    assert not bad.any(), (bad.sum().item(), x[bad.numpy()][:4])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_quantize_keeps_the_sign_of_zero(ctx, native, dtype):
     """Codes of zeros and of values that round to zero carry their sign, as a
