@@ -118,7 +118,8 @@ __device__ __forceinline__ void tmem_wait64(uint32_t (&r)[4][16]) {
 }
 
 // A tile of this CTA's shared memory to global memory (the map's box and swizzle);
-// rows and columns past the tensor's edges are not written.
+// rows past the tensor's edge are not written, nor columns past the 16 bytes
+// that its last column lies in.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -378,8 +379,8 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
     const float* scale = scales + half * C::BM + 32 * q + lane;
     uint32_t it = 0;
     bool ok = true, done = false, scaled = false;  // the next block's barriers, tested ahead
-    // Blocks of y sent so far, over all tiles: consecutive ones always take
-    // turns between the warp's two store blocks, so that all but the last
+    // Blocks of y sent by TMA so far, over all tiles: consecutive ones always
+    // take turns between the warp's two store blocks, so that all but the last
     // store being read is enough before a block is written again, even after
     // a tile that y's right edge left an odd number of blocks.
     uint32_t sends = 0;
@@ -444,19 +445,22 @@ __global__ void __launch_bounds__(ManyCfg::THREADS, 1)
       // 16 columns (f32) or 32 (16 bits) at a time: 64 bytes of each of the
       // warp's 32 rows go through shared memory, 16-byte chunk c of row r at
       // c ^ (r / 2 & 3), and out by TMA while the next ones are packed.
-      // Rows of y that do not start on 16-byte boundaries leave by plain
-      // stores, a warp's lanes side by side in a row.  (From the lane that
-      // holds the row, 8192 x 4096 -> 8192 took three times as long.)
+      // Rows of y that do not start on 16-byte boundaries, and the block that
+      // the last column ends inside 16 bytes (a TMA store writes the whole 16),
+      // leave by plain stores, a warp's lanes side by side in a row.  (From the
+      // lane that holds the row, 8192 x 4096 -> 8192 took three times as long.)
       auto send = [&](const uint4 (&o)[4], int col, int size) {
-        uint8_t* block = stage + (sends++ & 1) * C::EPI_BLOCK;
+        const bool tma = a.y_vec && (col + 64 / size <= a.out || a.out % (16 / size) == 0);
+        uint8_t* block = stage + (sends & 1) * C::EPI_BLOCK;
         if (lane == 0) tma_store_read_wait<1>();
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(block + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = o[i];
-        if (a.y_vec) {
+        if (tma) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) tma_store_2d(&my, block, col, (int)row0);
+          ++sends;
           return;
         }
         __syncwarp();

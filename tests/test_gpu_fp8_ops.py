@@ -452,6 +452,19 @@ def test_linear_last_tiles(ctx, rows, i, o, dtype, pad, off):
     assert torch.equal(y, exp.to(DT[dtype][1]))
 
 
+@pytest.mark.parametrize("rows,i,o", [(128 * 37, 640, 2048), (128 * 31, 300, 2001), (128 * 89, 384, 1024), (128 * 79 - 5, 700, 1001),
+                                      (128 * 111, 100, 500)])
+@pytest.mark.parametrize("dtype,pad,off", [("f32", 0, 0), ("f32", 7, 0), ("bf16", 7, 0), ("f16", 4, 4), ("bf16", 3, 1)])
+def test_linear_several_tiles_each(ctx, rows, i, o, dtype, pad, off):
+    """Two or more whole 128 x 256 tiles for a thread block (on 148 SMs), with
+    a last round that is full, whole, halved and quartered; widths that end
+    inside a 16-byte piece of rows with a stride of whole pieces.  Exact in
+    f32; rounded once otherwise."""
+    c, wc, sw, bias = linear_case(rows, i, o, rows + o, exact=True)
+    y = run_linear(ctx, c, wc, sw, bias, dtype, pad, off)
+    assert torch.equal(y, linear64(c, wc, sw, bias)[0].to(DT[dtype][1]))
+
+
 @pytest.mark.parametrize("rows,i,o,dtype", [(128 * 700, 128, 1000, "f32"), (128 * 700, 128, 800, "bf16"), (128 * 300, 128, 2344, "f32"),
                                             (128 * 460, 100, 40, "f32"), (128 * 460, 128, 24, "f16"), (128 * 75, 128, 1032, "f32")])
 def test_linear_odd_stores_then_more_tiles(ctx, rows, i, o, dtype):
