@@ -16,16 +16,18 @@
 //              distributed shared memory in rank order, so nothing depends on
 //              the order of arrival.
 //
-// What bounds them (B200, device time).  Many rows: 8192 x 4096 -> 8192 bf16
-// takes 257 us (2.14 PFLOP/s; 290 us and 1.9 PFLOP/s when repeated until the
-// power cap holds the clock; a bf16 library product of that size would take
-// 332 us at its measured 1.65 PFLOP/s).  The MMAs of a block take 512 cycles;
+// What bounds them (B200, device time in a captured graph, weights from HBM).
+// Many rows: 8192 x 4096 -> 8192 bf16 takes 259 us (2.12 PFLOP/s), in a stream
+// of calls, where the power cap holds the clock, 303 us (1.81 PFLOP/s); a bf16
+// library product of that size would take 332 us at its measured 1.65 PFLOP/s.
+// The MMAs of a block take 512 cycles;
 // its sums cross to the epilogue and back (issue 130, MMAs and their arrival
 // 600, loads and half of the sums 330, two wake-ups of about 200) in about
 // 1300 with two accumulators to hide them, and the f32 pipe is busy for 330.
-// TMEM holds no third accumulator of 256 columns.  A call of cut units alone
-// takes about 4 us and 0.26 us for each column block.  Few rows: 1 x 4096 ->
-// 32768 takes 25 us, 5.4 TB/s; below about 20 MB of weights a call is launch,
+// TMEM holds no third accumulator of 256 columns.  A call of quarter units alone
+// takes about 5 us and 0.26 us for each column block (100 x 1536 -> 6144 8.3 us,
+// 65 x 4096 -> 4096 13.6); halves take longer (512 x 4096 -> 4096 16.3).
+// Few rows: 1 x 4096 -> 32768 takes 24 us, 5.5 TB/s; below about 20 MB of weights a call is launch,
 // set-up (0.9 us), first bytes (0.8 us) and the cluster's exchange (0.7 us).
 //
 // Every mbarrier wait is bounded; a timeout records an error word and the
@@ -803,9 +805,9 @@ static cudaError_t launch_few(const Fp8GemmArgs& a, int sms, cudaStream_t st) {
   const long row_tiles = (a.rows + NT - 1) / NT, units = fp8_blocks(a.out) * row_tiles, kblocks = fp8_blocks(a.in);
   // Split the column blocks while the CTAs stay about as many as the SMs and
   // keep four blocks each, or fewer where they would leave most SMs idle.
-  // (1 x 4096 -> 4096: 11.7 us unsplit, 8.6 / 7.1 / 8.2 split by 2 / 4 / 8;
-  // 1 x 1536 -> 12288, 96 CTAs unsplit: 7.5, and 8.6 split by 2; 1 x 768 -> 768:
-  // 5.1, and 4.3 split by 4.)
+  // (1 x 4096 -> 4096: 11.3 us unsplit, 8.2 / 6.8 / 7.5 split by 2 / 4 / 8;
+  // 1 x 1536 -> 12288, 96 CTAs unsplit: 7.1, and 8.1 split by 2; 1 x 768 -> 768:
+  // 4.5, and 3.9 split by 4.)
   int lg = 0;
   while (lg < 3 && (units << (lg + 1)) <= sms + sms / 8 && (2 << lg) <= kblocks &&
          ((8 << lg) <= kblocks || (units << (lg + 3)) <= sms))
@@ -829,12 +831,12 @@ static cudaError_t launch_few(const Fp8GemmArgs& a, int sms, cudaStream_t st) {
 cudaError_t fp8_gemm(const Fp8GemmArgs& a, int dev, cudaStream_t st) {
   const int sms = g_num_sms(dev);
   // Up to 32 rows the weights are read once either way, and the few-rows
-  // kernel is the faster one (16 x 4096 -> 9000: 8.5 us, and 20.7 in tiles of
-  // 128 rows; 32 x 768 -> 2304: 5.6 and 5.2).  Beyond, only where it can split
-  // a long sum over clusters (100 x 4096 -> 1536: 9.7 and 12.3; 64 x 4096 ->
-  // 4096: 10.0 and 12.2), not unsplit (65 x 4096 -> 4096: 13.8 and 12.3; 100 x
-  // 1536 -> 6144: 9.2 and 7.2) nor for a short one (64 x 768 -> 768: 5.7 and
-  // 5.3).
+  // kernel is the faster one (16 x 4096 -> 9000: 10.4 us, and 22.9 in tiles of
+  // 128 rows; 32 x 768 -> 2304: 5.5 and 5.0).  Beyond, only where it can split
+  // a long sum over clusters (100 x 4096 -> 1536: 10.0 and 13.7; 64 x 4096 ->
+  // 4096: 10.6 and 13.8), not unsplit (65 x 4096 -> 4096: 13.7 and 13.6; 100 x
+  // 1536 -> 6144: 8.9 and 8.3) nor for a short one (64 x 768 -> 768: 5.5 and
+  // 5.2).
   if (a.rows <= 16) return launch_few<16>(a, sms, st);
   if (a.rows <= 32 || (fp8_blocks(a.in) >= 8 && fp8_blocks(a.out) * ((a.rows + 31) / 32) * 2 <= sms + sms / 8))
     return launch_few<32>(a, sms, st);
@@ -845,9 +847,9 @@ cudaError_t fp8_gemm(const Fp8GemmArgs& a, int dev, cudaStream_t st) {
   const long tiles = (a.rows + ManyCfg::BM - 1) / ManyCfg::BM * ((fp8_blocks(a.out) + 1) / 2);
   if (tiles > 0x3fffffffL) return cudaErrorInvalidValue;
   // What does not fill the SMs once more is cut to use them all: narrower
-  // units are done and stored sooner (2304 x 768 -> 2304, 148 + 14 tiles: 14.9
-  // us whole, 12.9 in halves, 12.2 in quarters; 512 x 4096 -> 4096, 64 tiles:
-  // 18.2 whole, 14.6 in halves).
+  // units are done and stored sooner (2304 x 768 -> 2304, 148 + 14 tiles: 15.3
+  // us whole, 13.2 in halves, 12.8 in quarters; 512 x 4096 -> 4096, 64 tiles:
+  // 19.1 whole, 16.3 in halves).
   const int rest = (int)(tiles % sms);
   const int lg = 4 * rest <= sms ? 2 : 2 * rest <= sms ? 1 : 0;
   const int full = (int)tiles - rest, grid = tiles >= sms ? sms : rest << lg;

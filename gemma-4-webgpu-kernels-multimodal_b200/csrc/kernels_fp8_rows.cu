@@ -13,10 +13,12 @@ namespace g4m {
 // Quantiser.  16 lanes hold one block (8 columns each): the block's largest
 // magnitude is four shuffles, and nothing else crosses lanes.  Half-warps
 // walk the blocks of all rows with the next block's loads in flight.  8192 x
-// 6144 bf16 with gelu (253 MB) takes 47 us, 5.3 TB/s, 0.82 of the measured
-// copy rate; silu 44.  Issue slots are close behind HBM (the sigmoid, the
-// rounded quotient): with magnitudes compared as integers it took 50 us, with
-// a warp-wide reduction in place of the four shuffles 49.
+// 6144 bf16 with gelu (253 MB) takes 49 us, 5.1 TB/s, 0.78 of the measured
+// copy rate (55 us in a stream of calls from Python); silu 47, without
+// activation (153 MB) 31.  Issue slots are close behind HBM (the sigmoid, the
+// rounded quotient): magnitudes compared as integers cost 2.7 us more, a
+// warp-wide reduction in place of the four shuffles 2.0.  Rows off 16-byte
+// boundaries, 8191 x 6143: 82 us with gelu, 47 without activation.
 // ---------------------------------------------------------------------------
 constexpr int kQuantThreads = 256;
 
@@ -104,9 +106,10 @@ cudaError_t fp8_quantize(const QuantArgs& a, int dev, cudaStream_t st) {
 // scales need no shared memory.  The two means of squares are the only row
 // sums.  Blocks walk the rows with the next row's loads in flight: with one
 // row per block, loads, sums and stores took turns.  16384 x 4096 (bf16 branch,
-// f32 residual, gate, codes out: 739 MB) takes 159 us, 4.7 TB/s, 0.71 of the
-// measured copy rate; to bf16 rows without gate 6.0 TB/s, 0.92.  Between them
-// stand the shuffles of the sums and block maxima and the rounded quotients.
+// f32 residual, gate, codes out: 739 MB) takes 157 us, 4.7 TB/s, 0.72 of the
+// measured copy rate; to bf16 rows without gate (537 MB) 96 us, 5.6 TB/s, 0.85.
+// Between them stand the shuffles of the sums and block maxima and the rounded
+// quotients.
 // ---------------------------------------------------------------------------
 struct NormKernelArgs {
   g4m_norm_args a;
@@ -160,6 +163,8 @@ __device__ __forceinline__ void scale8(float (&v)[8], float inv, const float* w,
 // threads with fewer chunks each, no loads ahead, and as many blocks as hide
 // each other's waits (2947 x 5193 bf16: 124 us with one block of 512 threads
 // an SM, 95 us with three of 384; 76 since row edges are stored by a mask).
+// Three such blocks leave a thread 56 registers: with two chunks 232 to 472
+// bytes of it spill, with one 16 to 104, by the types.
 template <int NCH, bool FULL>
 struct NormCfg {
   static constexpr int T = NCH == 4 ? 512 : FULL ? 256 : 384;

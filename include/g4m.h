@@ -116,15 +116,17 @@ G4M_API int g4m_linear_run_noalloc(g4m_linear* lin, const float* x_dev, int rows
  * linears are integer (src/kernels/qat.ts), its norms and rotary positions
  * live inside the towers (src/vision/kernels.ts:5-73).
  *
- * Common rules.  Every call is asynchronous on `stream` (NULL = the device's
- * legacy default stream) of device `device_index` of the context, allocates
- * nothing, keeps nothing between calls, can be captured into a graph, and
- * leaves the calling thread's current device as it was; calls on different
- * streams may overlap.  Row strides (ld*) are in elements, >= the row's
+ * Common rules.  Every call with a stream is asynchronous on `stream` (NULL =
+ * the device's legacy default stream) of device `device_index` of the context,
+ * allocates nothing, keeps nothing between calls and can be captured into a
+ * graph; calls on different streams may overlap.  The prepare calls allocate,
+ * upload and wait, the free calls free: none of them while a stream is being
+ * captured.  All leave the calling thread's current device as it was.  Row strides (ld*) are in elements, >= the row's
  * width, any alignment; pointers need the alignment of their element type
  * (G4M_E_ARG otherwise), 16-byte aligned rows are faster.  Zero rows are
  * G4M_OK and launch nothing.  Nothing outside the stated rows and columns is
  * read or written.  Inputs and outputs must not overlap except where stated.
+ * A repeated call gives the same bits, whatever runs beside it.
  * All are inference operators: none has a backward form.  None of them waits
  * for the device, so none reports a device-side wait that expired in an
  * earlier call: g4m_synchronize does. */
@@ -144,8 +146,8 @@ enum g4m_dtype { G4M_F32 = 0, G4M_BF16 = 1, G4M_F16 = 2 };
  * codes is 16-byte aligned and ldc a multiple of 16 (the linear fetches the
  * rows by TMA); scales hold ceil(columns / 128) runs of lds >= rows floats.
  * The quantising operators choose scale = max(amax, 2^-96) / 448 from the
- * block's largest magnitude and code = e4m3(value / scale), to nearest even.
- * A block that holds a NaN or an infinity gets a NaN scale and NaN codes. */
+ * block's largest magnitude and code = e4m3(value / scale), to nearest even of
+ * the f32 quotient, zeros with their sign.  A block that holds a NaN or an infinity gets a NaN scale and NaN codes. */
 typedef struct g4m_fp8_rows {
   uint8_t* codes;
   int64_t ldc;
@@ -174,7 +176,9 @@ G4M_API int g4m_fp8_linear_prepare(g4m_ctx* ctx, int device_index, const uint8_t
                                    const float* bias, g4m_fp8_linear** out_linear);
 /* y[r][o] = sum over blocks k of 128 columns of
  *             (sum of code products in block k) * scale_x[k][r] * w_scales[o / 128][k]   (+ bias[o])
- * summed in f32, rounded once to y_dtype.  x holds `rows` rows of `in` columns. */
+ * summed in f32, rounded once to y_dtype.  x holds `rows` rows of `in` columns.
+ * The number of rows decides how the sum over k is cut and where the bias
+ * joins it, so the last bits of a row depend on how many rows the call has. */
 G4M_API int g4m_fp8_linear_run(g4m_fp8_linear* lin, const g4m_fp8_rows* x, int64_t rows, void* y, int y_dtype, int64_t ldy,
                                void* stream);
 G4M_API void g4m_fp8_linear_free(g4m_fp8_linear* lin);
@@ -218,7 +222,8 @@ G4M_API int g4m_norm_residual(g4m_ctx* ctx, int device_index, const g4m_norm_arg
  * with (u, v) = elements (j, j + rotary/2) of the head (interleaved == 0) or
  * (2 j, 2 j + 1) (interleaved != 0), j < rotary/2; elements from `rotary` on
  * pass through unscaled.  The angle is formed modulo one turn from a 64-bit
- * fixed-point frequency, so far positions lose nothing. */
+ * fixed-point frequency: off by at most |position| * 2^-65 turns (2^-25 turns
+ * at 2^40).  Its distance from the nearest quarter turn is then rounded to f32. */
 enum g4m_rope_scaling {
   G4M_ROPE_NONE = 0,    /* theta^(-2 j / rotary) */
   G4M_ROPE_LINEAR = 1,  /* the same / factor */
