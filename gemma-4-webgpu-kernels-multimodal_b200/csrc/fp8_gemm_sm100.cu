@@ -20,15 +20,15 @@
 // Many rows: 8192 x 4096 -> 8192 bf16 takes 259 us (2.12 PFLOP/s), in a stream
 // of calls, where the power cap holds the clock, 303 us (1.81 PFLOP/s); a bf16
 // library product of that size would take 332 us at its measured 1.65 PFLOP/s.
-// The MMAs of a block take 512 cycles;
-// its sums cross to the epilogue and back (issue 130, MMAs and their arrival
-// 600, loads and half of the sums 330, two wake-ups of about 200) in about
-// 1300 with two accumulators to hide them, and the f32 pipe is busy for 330.
-// TMEM holds no third accumulator of 256 columns.  A call of quarter units alone
-// takes about 5 us and 0.26 us for each column block (100 x 1536 -> 6144 8.3 us,
-// 65 x 4096 -> 4096 13.6); halves take longer (512 x 4096 -> 4096 16.3).
-// Few rows: 1 x 4096 -> 32768 takes 24 us, 5.5 TB/s; below about 20 MB of weights a call is launch,
-// set-up (0.9 us), first bytes (0.8 us) and the cluster's exchange (0.7 us).
+// The MMAs of a block take 512 cycles; its sums cross to the epilogue and back
+// (issue 130, MMAs and their arrival 600, loads and half of the sums 330, two
+// wake-ups of about 200) in about 1300 with two accumulators to hide them, and
+// the f32 pipe is busy for 330.  TMEM holds no third accumulator of 256
+// columns.  A call of quarter units alone takes about 5 us and 0.26 us for
+// each column block (100 x 1536 -> 6144 8.3 us, 65 x 4096 -> 4096 13.6);
+// halves take longer (512 x 4096 -> 4096 16.3).  Few rows: 1 x 4096 -> 32768
+// takes 24 us, 5.5 TB/s; below about 20 MB of weights a call is launch, set-up
+// (0.9 us), first bytes (0.8 us) and the cluster's exchange (0.7 us).
 //
 // Every mbarrier wait is bounded; a timeout records an error word and the
 // CTA unwinds.

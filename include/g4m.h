@@ -121,15 +121,15 @@ G4M_API int g4m_linear_run_noalloc(g4m_linear* lin, const float* x_dev, int rows
  * allocates nothing, keeps nothing between calls and can be captured into a
  * graph; calls on different streams may overlap.  The prepare calls allocate,
  * upload and wait, the free calls free: none of them while a stream is being
- * captured.  All leave the calling thread's current device as it was.  Row strides (ld*) are in elements, >= the row's
- * width, any alignment; pointers need the alignment of their element type
- * (G4M_E_ARG otherwise), 16-byte aligned rows are faster.  Zero rows are
- * G4M_OK and launch nothing.  Nothing outside the stated rows and columns is
- * read or written.  Inputs and outputs must not overlap except where stated.
- * A repeated call gives the same bits, whatever runs beside it.
- * All are inference operators: none has a backward form.  None of them waits
- * for the device, so none reports a device-side wait that expired in an
- * earlier call: g4m_synchronize does. */
+ * captured.  All leave the calling thread's current device as it was.  Row
+ * strides (ld*) are in elements, >= the row's width, any alignment; pointers
+ * need the alignment of their element type (G4M_E_ARG otherwise), 16-byte
+ * aligned rows are faster.  Zero rows are G4M_OK and launch nothing.  Nothing
+ * outside the stated rows and columns is read or written.  Inputs and outputs
+ * must not overlap except where stated.  A repeated call gives the same bits,
+ * whatever runs beside it.  All are inference operators: none has a backward
+ * form.  None of them waits for the device, so none reports a device-side wait
+ * that expired in an earlier call: g4m_synchronize does. */
 
 /* Wait for `stream` (NULL = the device's legacy default stream; not one that
  * is being captured).  G4M_E_TIMEOUT when a bounded wait of any kernel on the
@@ -147,7 +147,8 @@ enum g4m_dtype { G4M_F32 = 0, G4M_BF16 = 1, G4M_F16 = 2 };
  * rows by TMA); scales hold ceil(columns / 128) runs of lds >= rows floats.
  * The quantising operators choose scale = max(amax, 2^-96) / 448 from the
  * block's largest magnitude and code = e4m3(value / scale), to nearest even of
- * the f32 quotient, zeros with their sign.  A block that holds a NaN or an infinity gets a NaN scale and NaN codes. */
+ * the f32 quotient, zeros with their sign.  A block that holds a NaN or an
+ * infinity gets a NaN scale and NaN codes. */
 typedef struct g4m_fp8_rows {
   uint8_t* codes;
   int64_t ldc;

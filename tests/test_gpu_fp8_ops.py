@@ -1002,6 +1002,51 @@ def test_profile_counts_every_thread(ctx, native):
         layer.check()
 
 
+def test_beside_a_tower_call(native, syn, tmp_path):
+    """Layers on two streams while another thread embeds images with the same
+    context: all give what they give alone."""
+    import threading
+    path = str(tmp_path / "v.safetensors")
+    syn.write_safetensors(path, syn.vision_weights(0, layers=2))
+    c = native.Context()
+    try:
+        c.load_weights(path)
+        pix = [syn.image_pixels(k, 768, 768) for k in range(3)]
+        layers = [Layer(c, native, 24, 40), Layer(c, native, 2000, 41)]
+        outs, _ = c.vision_embed(pix, 256, 2)
+        want = []
+        for layer in layers:
+            layer.run()
+            torch.cuda.synchronize()
+            want.append(layer.outputs())
+        got, failed = [], []
+
+        def tower():
+            try:
+                for _ in range(4):
+                    got.append(c.vision_embed(pix, 256, 2)[0])
+            except Exception as e:  # a thread's exception would be lost
+                failed.append(repr(e))
+
+        t = threading.Thread(target=tower)
+        t.start()
+        streams = [torch.cuda.Stream() for _ in layers]
+        for _ in range(40):
+            for layer, s in zip(layers, streams):
+                with torch.cuda.stream(s):
+                    layer.run()
+        t.join()
+        torch.cuda.synchronize()
+        assert not failed, failed
+        for layer, exp in zip(layers, want):
+            assert all(torch.equal(p, q) for p, q in zip(layer.outputs(), exp))
+        for again in got:
+            assert all(np.array_equal(p, q) for p, q in zip(again, outs))
+        c.synchronize()
+    finally:
+        c.close()
+
+
 def test_default_stream_is_the_legacy_one(ctx):
     """Stream 0 orders with torch's default stream."""
     x = torch.zeros(64, 4096, device="cuda")
